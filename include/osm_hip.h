@@ -176,6 +176,13 @@ int osm_q4_projection_create(osm_context ctx, const uint32_t* packed, size_t pac
                              size_t out_dim, size_t packed_cols, const void* scales,
                              const void* biases, uint32_t meta_dtype, size_t group_size,
                              osm_q4_projection* out);
+/* The same handle over arrays that are on the device already: packed
+ * [out_dim, packed_cols], scales and biases [out_dim, packed_cols * 8 /
+ * group_size], each 16-byte aligned. Nothing is copied; the caller keeps them
+ * alive and unchanged while calls that use the handle run. */
+int osm_q4_projection_on_device(osm_context ctx, const uint32_t* packed_dev, size_t out_dim,
+                                size_t packed_cols, const void* scales_dev, const void* biases_dev,
+                                uint32_t meta_dtype, size_t group_size, osm_q4_projection* out);
 void osm_q4_projection_destroy(osm_q4_projection p);
 /* run_vulkan_q4_gemv_preloaded (vulkan_q4_gemv.hpp:53-57). */
 int osm_q4_gemv_preloaded(osm_context ctx, osm_q4_projection weights, osm_buffer x, osm_buffer y);
@@ -185,6 +192,75 @@ int osm_swiglu_buffers(osm_context ctx, osm_buffer gate, osm_buffer up, osm_buff
  * accumulator[i] += weight * source[i]. */
 int osm_weighted_accumulate(osm_context ctx, osm_buffer source, float weight,
                             osm_buffer accumulator);
+
+/* ---- operators of batches ----------------------------------------------------
+ * No counterpart in the reference, which routes one way and projects one
+ * vector at a time. Device pointers in and out, ordered on the context's
+ * stream, no synchronisation; they may be captured into a graph. A call of 0
+ * tokens or rows is valid (row grouping still writes its offsets). Arrays
+ * are on the context's device, outputs do not overlap inputs, and host
+ * structures are read before the call returns.
+ *
+ * Routing to experts by a rule. Row t of logits [tokens, E] (F32, F16 or
+ * BF16, rows logits_stride elements apart, 0 for E) gives
+ *   scores   s_e: softmax over the E logits, or 1 / (1 + exp(-l_e));
+ *   choices  c_e = s_e + bias_e (bias [E] fp32, or NULL for none);
+ *   groups   of E / groups consecutive experts: those with the top_groups best
+ *            sums of their best group_score choices stay (ties: lower group);
+ *   ids      [tokens, k] the best choices in the groups that stay, in
+ *            descending order, ties to the lower id;
+ *   weights  [tokens, k] scale * s / (renormalize ? the picks' sum of s : 1);
+ *   mass     [tokens] the picks' sum of s (NULL for none).
+ * Scores are computed and compared in fp64; without a bias experts are ranked
+ * by their logits, which is the same order without its roundings. A logit of
+ * -infinity or NaN, or a choice that is, makes an expert unavailable: where
+ * fewer than k are left, the remaining picks are the lowest other ids, with
+ * weight 0. A sum of 0 gives weights of 0. */
+enum osm_route_score { OSM_SCORE_SOFTMAX = 0, OSM_SCORE_SIGMOID = 1 };
+typedef struct osm_route_rule {
+  uint32_t expert_count; /* E, in [1, 1024] */
+  uint32_t top_k;        /* k, in [1, 64], at most top_groups * E / groups */
+  uint32_t score;        /* OSM_SCORE_* */
+  uint32_t groups;       /* in [1, 64], dividing E; 1: no groups */
+  uint32_t top_groups;   /* in [1, groups] */
+  uint32_t group_score;  /* 1 or 2, at most E / groups */
+  uint32_t renormalize;
+  float scale;           /* finite */
+} osm_route_rule;
+int osm_route_experts(osm_context ctx, const osm_route_rule* rule, const void* logits_dev,
+                      uint32_t logits_dtype, size_t logits_stride, const float* bias_dev,
+                      uint32_t tokens, uint32_t* ids_dev, float* weights_dev, float* mass_dev);
+/* Rows grouped by key, stable: order [rows] lists the rows of key 0, then of
+ * key 1, ..., then those whose key is outside [0, buckets), each in row order;
+ * offsets [buckets + 1] say where each key's rows start (the last entry: where
+ * the rows outside do). Groups (token, expert) pairs by expert, or a batch's
+ * tokens by adapter. buckets in [1, 65535]. */
+int osm_group_rows(osm_context ctx, const int32_t* keys_dev, uint32_t rows, uint32_t buckets,
+                   uint32_t* offsets_dev, uint32_t* order_dev);
+/* Low-rank adapters of one projection, in device memory of the caller's.
+ * Adapter i has rank ranks[i] (NULL, or beyond max_rank: max_rank): rows
+ * below it of a[i] and columns below it of b[i] count, the rest is not used. */
+typedef struct osm_adapters {
+  const void* a;         /* [count, max_rank, in_dim] */
+  const void* b;         /* [count, out_dim, max_rank] */
+  const float* scales;   /* [count], or NULL for 1 */
+  const uint32_t* ranks; /* [count], or NULL */
+  uint32_t count;        /* at least 1 */
+  uint32_t max_rank;     /* in [1, 256] */
+  uint32_t dtype;        /* OSM_F32 / OSM_F16 / OSM_BF16 of a and b */
+} osm_adapters;
+/* A q4 projection of `tokens` rows, each with its own adapter beside it:
+ *   y_t = W x_t + scales[i] * b[i] (a[i] x_t),  i = adapter_ids[t]
+ * (nothing beside W x_t where i is outside [0, count), or with adapters
+ * NULL). x [tokens, in_dim] and y [tokens, out_dim] are F32, F16 or BF16, rows
+ * x_stride / y_stride elements apart (0: dense). Sums are fp32; y is rounded
+ * once. x is finite: a row that is not gives unspecified values in its own
+ * row of y, and in no other. At most 2^20 tokens a call. It works in the
+ * context's shared workspace, which cannot grow while a capture is recording:
+ * make the call, or a larger one, once before. */
+int osm_q4_project(osm_context ctx, osm_q4_projection weights, const void* x_dev, uint32_t x_dtype,
+                   size_t x_stride, void* y_dev, uint32_t y_dtype, size_t y_stride, uint32_t tokens,
+                   const osm_adapters* adapters, const int32_t* adapter_ids_dev);
 
 /* ---- experts ----------------------------------------------------------------
  * Blob size of one expert (docs/OSM-39B-QPACK-EXPERT-GEOMETRY.md:61-74 byte
@@ -319,6 +395,16 @@ uint32_t osm_moe_layer_static_tokens_capacity(osm_moe_layer l);
  * by expert and reads each expert once. */
 enum osm_moe_path { OSM_PATH_AUTO = 0, OSM_PATH_PER_TOKEN = 1, OSM_PATH_GROUPED = 2 };
 int osm_moe_layer_set_path(osm_moe_layer l, int path);
+/* Routes the layer's further calls by a rule (osm_route_experts on the
+ * device's own logits) instead of by softmax top-k: every path, cached and
+ * static calls and graphs recorded from then on. expert_count and top_k are
+ * the layer's; norm_topk_prob gives way to the rule's renormalize. bias: host
+ * [expert_count] or NULL; graphs recorded with one use the layer's last. rule
+ * NULL: softmax top-k again. Not while a capture is recording. The reference
+ * has no such routing, so nothing is recomputed in its order, and logits that
+ * two paths sum differently may rank differently where they all but tie. */
+int osm_moe_layer_set_routing(osm_context ctx, osm_moe_layer l, const osm_route_rule* rule,
+                              const float* bias);
 /* A prefill chunk: bf16 x [tokens, D] (device, 16-byte aligned) through the
  * grouped path, MoE form, y fp32 [tokens, D]; needs a bf16 router. Routing
  * per token is that of run_qwen_sparse_moe_vulkan_accum on the widened x. */
@@ -399,7 +485,7 @@ int osm_moe_decode_layers(osm_context ctx, const osm_moe_layer* layers,
  * launches; layers, slabs and buffers must outlive the graph. Between
  * capture_begin and capture_end only enqueue-only calls may be made on the
  * context (decode_layers, moe_layer_decode_device, moe_layer_launch_phase,
- * memcpy_d2d_async); capture_end always ends the capture. */
+ * memcpy_d2d_async, and the operators of batches); capture_end always ends the capture. */
 int osm_decode_graph_create(osm_context ctx, const osm_moe_layer* layers,
                             const uint32_t* slab_layers, uint32_t n_layers, osm_expert_slab slab,
                             const float* x_dev, float* y_dev, float* scratch_dev, uint32_t tokens,

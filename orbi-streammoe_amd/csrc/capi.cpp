@@ -434,6 +434,19 @@ int osm_q4_projection_create(osm_context ctx, const uint32_t* packed, size_t pac
   return ok();
   OSM_GUARD_END
 }
+int osm_q4_projection_on_device(osm_context ctx, const uint32_t* packed_dev, size_t out_dim, size_t packed_cols,
+                                const void* scales_dev, const void* biases_dev, uint32_t meta_dtype, size_t group_size,
+                                osm_q4_projection* out) {
+  OSM_GUARD_BEGIN
+  if (!ctx || !out) return fail(OSM_E_INVALID, "null argument");
+  std::string d;
+  auto w = osm::HipQ4ProjectionWeights::on_device(ctx->ctx, packed_dev, out_dim, packed_cols, scales_dev, biases_dev,
+                                                  meta_dtype, group_size, &d);
+  if (!w) return fail(OSM_E_INVALID, d);
+  *out = new osm_q4_projection_s{std::move(*w)};
+  return ok();
+  OSM_GUARD_END
+}
 void osm_q4_projection_destroy(osm_q4_projection p) { delete p; }
 
 int osm_q4_gemv_preloaded(osm_context ctx, osm_q4_projection weights, osm_buffer x, osm_buffer y) {
@@ -449,6 +462,58 @@ int osm_swiglu_buffers(osm_context ctx, osm_buffer gate, osm_buffer up, osm_buff
 int osm_weighted_accumulate(osm_context ctx, osm_buffer source, float weight, osm_buffer accumulator) {
   if (!ctx || !source || !accumulator) return fail(OSM_E_INVALID, "null argument");
   auto r = osm::run_hip_weighted_accumulate(ctx->ctx, source->buf, weight, accumulator->buf);
+  return from_diag(r.executed, r.diagnostic);
+}
+
+// ---- operators of batches ----------------------------------------------------
+namespace {
+osm::HipRouteRule rule_of(const osm_route_rule& r) {
+  osm::HipRouteRule out;
+  out.expert_count = r.expert_count;
+  out.top_k = r.top_k;
+  out.score = r.score;
+  out.groups = r.groups;
+  out.top_groups = r.top_groups;
+  out.group_score = r.group_score;
+  out.renormalize = r.renormalize != 0U;
+  out.scale = r.scale;
+  return out;
+}
+}  // namespace
+
+int osm_route_experts(osm_context ctx, const osm_route_rule* rule, const void* logits_dev, uint32_t logits_dtype,
+                      size_t logits_stride, const float* bias_dev, uint32_t tokens, uint32_t* ids_dev,
+                      float* weights_dev, float* mass_dev) {
+  if (!ctx || !rule) return fail(OSM_E_INVALID, "null argument");
+  auto r = osm::run_hip_route_experts(ctx->ctx, rule_of(*rule), logits_dev, logits_dtype, logits_stride, bias_dev,
+                                      tokens, ids_dev, weights_dev, mass_dev);
+  return from_diag(r.executed, r.diagnostic);
+}
+
+int osm_group_rows(osm_context ctx, const int32_t* keys_dev, uint32_t rows, uint32_t buckets, uint32_t* offsets_dev,
+                   uint32_t* order_dev) {
+  if (!ctx) return fail(OSM_E_INVALID, "null argument");
+  auto r = osm::run_hip_group_rows(ctx->ctx, keys_dev, rows, buckets, offsets_dev, order_dev);
+  return from_diag(r.executed, r.diagnostic);
+}
+
+int osm_q4_project(osm_context ctx, osm_q4_projection weights, const void* x_dev, uint32_t x_dtype, size_t x_stride,
+                   void* y_dev, uint32_t y_dtype, size_t y_stride, uint32_t tokens, const osm_adapters* adapters,
+                   const int32_t* adapter_ids_dev) {
+  if (!ctx || !weights) return fail(OSM_E_INVALID, "null argument");
+  osmd_adapters ad{};
+  if (adapters) {
+    if (adapters->count == 0U) return fail(OSM_E_INVALID, "Q4 projection: adapters with a count of zero");
+    ad.a = adapters->a;
+    ad.b = adapters->b;
+    ad.scales = adapters->scales;
+    ad.ranks = adapters->ranks;
+    ad.count = adapters->count;
+    ad.max_rank = adapters->max_rank;
+    ad.dtype = adapters->dtype;
+  }
+  auto r = osm::run_hip_q4_project(ctx->ctx, weights->w, x_dev, x_dtype, x_stride, y_dev, y_dtype, y_stride, tokens, ad,
+                                   adapter_ids_dev);
   return from_diag(r.executed, r.diagnostic);
 }
 
@@ -811,6 +876,18 @@ void osm_graph_destroy(osm_graph g) { delete g; }
 }  // extern "C"
 
 extern "C" {
+
+int osm_moe_layer_set_routing(osm_context ctx, osm_moe_layer l, const osm_route_rule* rule, const float* bias) {
+  OSM_GUARD_BEGIN
+  if (!ctx || !l) return fail(OSM_E_INVALID, "null argument");
+  std::string d;
+  if (!rule) return l->layer.set_routing(ctx->ctx, nullptr, {}, &d) ? ok() : fail(OSM_E_INVALID, d);
+  const osm::HipRouteRule r = rule_of(*rule);
+  const std::span<const float> b = bias ? std::span<const float>(bias, l->layer.config().expert_count)
+                                        : std::span<const float>();
+  return l->layer.set_routing(ctx->ctx, &r, b, &d) ? ok() : fail(OSM_E_INVALID, d);
+  OSM_GUARD_END
+}
 
 int osm_moe_layer_set_path(osm_moe_layer l, int path) {
   if (!l) return fail(OSM_E_INVALID, "null layer");

@@ -2717,6 +2717,7 @@ RouteView route_view(const osmd_moe_args& a) {
 }
 
 int launch_select(const osmd_moe_args& a, hipStream_t st) {
+  if (a.rule.active) return osmd_moe_select_rule(&a, st);
   const RouteView rv = route_view(a);
   // ExactMode. In the sublayer form the clusters need rows that the split
   // chains take; others, up to 1,024 tokens, run the deep form.
@@ -2827,6 +2828,11 @@ int osmd_moe_route(const osmd_moe_args* a, osmd_stream s) {
 }
 
 int osmd_moe_gate_up(const osmd_moe_args* a, osmd_stream s) {
+  if (a->expert_table && a->rule.active) {
+    // A rule selects in its own launch, and gate/up reads its slot pointers.
+    const int r = osmd_moe_select_rule(a, s);
+    return r != 0 ? r : launch_gate_up(gate_up_params(*a), a->tokens, 0, static_cast<hipStream_t>(s));
+  }
   const int per = a->expert_table ? selection_per(a->expert_count) : 0;
   // gate/up's own selection reads final logits (the per-token router's);
   // router GEMM planes go through the select kernel.

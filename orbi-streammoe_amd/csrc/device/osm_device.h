@@ -81,6 +81,9 @@ int osmd_capture_end(osmd_stream s, osmd_graph* out);
 int osmd_graph_launch(osmd_graph g, osmd_stream s);
 int osmd_graph_destroy(osmd_graph g);
 
+/* Whether a capture is recording on the stream (allocations would end it). */
+int osmd_stream_capturing(osmd_stream s, int* capturing);
+
 /* ---- elementwise / projection kernels ----------------------------------- */
 typedef struct osmd_q4_proj {
   const uint32_t* packed; /* [out_dim, packed_cols] */
@@ -123,6 +126,19 @@ enum {
   OSMD_MOE_RESIDUAL = 2u, /* y = x + moe(norm(x)) */
   OSMD_MOE_SHARED = 4u    /* add the sigmoid-gated shared expert */
 };
+
+/* Routing by a rule (osmd_route_experts; a layer's when `active`). */
+enum { OSMD_SCORE_SOFTMAX = 0u, OSMD_SCORE_SIGMOID = 1u };
+typedef struct osmd_route_rule {
+  uint32_t active;      /* osmd_moe_args: select by this rule */
+  uint32_t score;       /* OSMD_SCORE_* */
+  uint32_t groups;      /* groups of E / groups consecutive experts; 1: none */
+  uint32_t top_groups;  /* groups that stay */
+  uint32_t group_score; /* a group's score: the sum of its best 1 or 2 choices */
+  uint32_t renormalize; /* divide the picks' scores by their sum */
+  float scale;          /* factor of the weights */
+  const float* bias;    /* [E] device, added to the scores for the choice alone; or null */
+} osmd_route_rule;
 
 typedef struct osmd_moe_args {
   osm_expert_geometry geom;
@@ -172,6 +188,10 @@ typedef struct osmd_moe_args {
   const float* bound_planes;
   uint32_t* route_stats;
   uint32_t x_bf16;
+  /* When rule.active the selection goes by it (osmd_moe_select_rule), on the
+   * device's logits as they are: the reference has no such routing to be
+   * exact against, so no bounds and no exact path. */
+  osmd_route_rule rule;
 } osmd_moe_args;
 
 /* Largest top-k and expert count the fused decode kernels accept. */
@@ -199,6 +219,45 @@ int osmd_moe_down(const osmd_moe_args* a, osmd_stream s);
 /* The selection kernel alone: top-k of a->logits for a->tokens tokens into
  * ids / weights / mass (and slot_ptrs from expert_table when set). */
 int osmd_moe_select(const osmd_moe_args* a, osmd_stream s);
+
+/* Routing by a rule: logits [tokens, experts] of OSM_META_F32 / F16 / BF16,
+ * rows `stride` elements apart, to ids / weights [tokens, top_k] and (may be
+ * null) the picks' score sum [tokens]. osmd_moe_select_rule is the layer's
+ * selection with a->rule: also the planes' sums, slot pointers and counter. */
+#define OSMD_ROUTE_MAX_TOP_K 64u
+int osmd_route_experts(const osmd_route_rule* rule, const void* logits, uint32_t dtype, size_t stride, uint32_t tokens,
+                       uint32_t experts, uint32_t top_k, uint32_t* ids, float* weights, float* mass, osmd_stream s);
+int osmd_moe_select_rule(const osmd_moe_args* a, osmd_stream s);
+
+/* Rows grouped by key, stable: order [rows] holds the rows of key 0, of key
+ * 1, ..., then those whose key is outside [0, buckets); offsets [buckets + 1]
+ * where each starts (the last: where the rows outside start). */
+#define OSMD_GROUP_MAX_BUCKETS 65535u
+int osmd_group_rows(const int32_t* keys, uint32_t rows, uint32_t buckets, uint32_t* offsets, uint32_t* order,
+                    osmd_stream s);
+
+/* y = W x + scale_a B_a (A_a x) for tokens rows, a = adapter_ids[token] (none
+ * outside [0, count)). v [tokens, max_rank] fp32 scratch (adapters only). */
+typedef struct osmd_adapters {
+  const void* a;          /* [count, max_rank, in_dim] */
+  const void* b;          /* [count, out_dim, max_rank] */
+  const float* scales;    /* [count] or null (1) */
+  const uint32_t* ranks;  /* [count] or null (max_rank) */
+  uint32_t count, max_rank, dtype; /* dtype: OSM_META_* of a and b */
+} osmd_adapters;
+typedef struct osmd_project_args {
+  osmd_q4_proj w;
+  const void* x;
+  void* y;
+  size_t x_stride, y_stride; /* elements between rows */
+  uint32_t x_dtype, y_dtype; /* OSM_META_* */
+  uint32_t tokens;
+  osmd_adapters adapters;    /* count 0: none */
+  const int32_t* adapter_ids;
+} osmd_project_args;
+#define OSMD_MAX_ADAPTER_RANK 256u
+size_t osmd_q4_project_workspace(const osmd_project_args* a);
+int osmd_q4_project(const osmd_project_args* a, void* workspace, osmd_stream s);
 
 /* Host-driven residency in rounds (a capped cache runs some slots before
  * others are resident: picks that are already resident while the rest are

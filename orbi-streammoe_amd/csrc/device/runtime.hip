@@ -160,6 +160,12 @@ int osmd_stream_device(osmd_stream s, int* device) {
 int osmd_stream_destroy(osmd_stream s) {
   return s ? rc(hipStreamDestroy(static_cast<hipStream_t>(s))) : 0;
 }
+int osmd_stream_capturing(osmd_stream s, int* capturing) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  const int r = rc(hipStreamIsCapturing(static_cast<hipStream_t>(s), &st));
+  *capturing = st == hipStreamCaptureStatusNone ? 0 : 1;
+  return r;
+}
 int osmd_stream_synchronize(osmd_stream s) {
   return rc(hipStreamSynchronize(static_cast<hipStream_t>(s)));
 }

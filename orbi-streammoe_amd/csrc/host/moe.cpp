@@ -153,6 +153,9 @@ struct HipMoeLayer::Impl {
   // grouped (multi-token) path: carved per call from the context's shared
   // workspace (every layer on one stream uses the same memory in turn)
   HipMoePath path = HipMoePath::automatic;
+  // Selection by a rule (set_routing); rule.bias points into rule_bias.
+  osmd_route_rule rule{};
+  DeviceBytes rule_bias;
   enum GroupedBuf { kXTerms, kXSums, kPairPos, kPairW, kTiles, kTileCount, kGuPart, kHTerms, kHSums, kPartial,
                     kLogitPlanes, kXNorms, kBoundPlanes, kGroupedBufs };
   std::array<std::size_t, kGroupedBufs> g_off{};
@@ -272,6 +275,7 @@ struct HipMoeLayer::Impl {
     a.x_norm = x_norm.as<float>();
     a.h = h.as<float>();
     a.slot_ptrs = slot_ptrs.as<const std::uint8_t*>();
+    a.rule = rule;
     return a;
   }
 };
@@ -592,6 +596,50 @@ bool HipMoeLayer::set_path(HipMoePath path, std::string* diagnostic) noexcept {
     return set_diag(diagnostic, "unknown MoE path"), false;
   impl_->path = path;
   return true;
+}
+
+bool HipMoeLayer::set_routing(HipComputeContext& context, const HipRouteRule* rule, std::span<const float> bias,
+                              std::string* diagnostic) noexcept {
+  try {
+    if (!valid()) return set_diag(diagnostic, "MoE layer is not valid"), false;
+    if (rule == nullptr) {
+      impl_->rule.active = 0U;
+      return true;
+    }
+    if (!check_route_rule(*rule, diagnostic)) return false;
+    if (rule->expert_count != impl_->cfg.expert_count || rule->top_k != impl_->cfg.top_k)
+      return set_diag(diagnostic, "routing rule: expert_count and top_k must be the layer's"), false;
+    if (!bias.empty() && bias.size() != impl_->cfg.expert_count)
+      return set_diag(diagnostic, "routing rule: the bias must have expert_count values"), false;
+    for (float b : bias)
+      if (std::isnan(b)) return set_diag(diagnostic, "routing rule: the bias contains NaN"), false;
+    if (!context.activate(diagnostic)) return false;
+    if (context.device() != impl_->device)
+      return set_diag(diagnostic, "MoE layer belongs to a different device"), false;
+    int capturing = 0;
+    if (osmd_stream_capturing(context.stream(), &capturing) != 0 || capturing)
+      return set_diag(diagnostic, "routing rule: cannot be set while a capture is recording on the stream"), false;
+    if (!bias.empty()) {
+      // One buffer for the layer's life: graphs captured with a bias read the
+      // one set last.
+      int rc = impl_->rule_bias.get() ? 0 : impl_->rule_bias.allocate(bias.size_bytes());
+      if (rc == 0) rc = osmd_memcpy_h2d(impl_->rule_bias.get(), bias.data(), bias.size_bytes(), context.stream());
+      if (rc == 0) rc = osmd_stream_synchronize(context.stream());
+      if (rc != 0) return set_diag(diagnostic, hip_error("routing bias upload failed", rc)), false;
+    }
+    osmd_route_rule& r = impl_->rule;
+    r.active = 1U;
+    r.score = rule->score;
+    r.groups = rule->groups;
+    r.top_groups = rule->top_groups;
+    r.group_score = rule->group_score;
+    r.renormalize = rule->renormalize ? 1U : 0U;
+    r.scale = rule->scale;
+    r.bias = bias.empty() ? nullptr : impl_->rule_bias.as<const float>();
+    return true;
+  } catch (const std::exception& e) {
+    return set_diag(diagnostic, std::string("routing rule exception: ") + e.what()), false;
+  }
 }
 
 HipMoePath HipMoeLayer::path() const noexcept { return impl_ ? impl_->path : HipMoePath::automatic; }

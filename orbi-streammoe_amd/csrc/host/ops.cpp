@@ -55,7 +55,10 @@ bool same_device(const HipComputeContext& ctx, int dev) { return ctx.valid() && 
 
 // ---- HipQ4ProjectionWeights ------------------------------------------------
 struct HipQ4ProjectionWeights::Impl {
-  DeviceBytes packed, scales, biases;
+  DeviceBytes packed, scales, biases;  // owned arrays; empty for a caller's
+  const std::uint32_t* packed_at = nullptr;
+  const void* scales_at = nullptr;
+  const void* biases_at = nullptr;
   std::size_t out_dim = 0, packed_cols = 0, group = 0;
   std::uint32_t meta_dtype = OSM_META_F32;
   int device = -1;
@@ -108,6 +111,9 @@ std::optional<HipQ4ProjectionWeights> HipQ4ProjectionWeights::create_raw(
       set_diag(diagnostic, hip_error("Q4 projection upload failed", rc));
       return std::nullopt;
     }
+    impl->packed_at = impl->packed.as<const std::uint32_t>();
+    impl->scales_at = impl->scales.get();
+    impl->biases_at = impl->biases.get();
     impl->out_dim = out_dim;
     impl->packed_cols = packed_cols;
     impl->group = group_size;
@@ -123,23 +129,66 @@ std::optional<HipQ4ProjectionWeights> HipQ4ProjectionWeights::create_raw(
   }
 }
 
-bool HipQ4ProjectionWeights::valid() const noexcept { return impl_ && impl_->packed.get(); }
+std::optional<HipQ4ProjectionWeights> HipQ4ProjectionWeights::on_device(
+    HipComputeContext& context, const std::uint32_t* packed, std::size_t out_dim, std::size_t packed_cols,
+    const void* scales, const void* biases, std::uint32_t meta_dtype, std::size_t group_size,
+    std::string* diagnostic) noexcept {
+  try {
+    if (!context.valid()) return set_diag(diagnostic, "HIP compute context is not valid"), std::nullopt;
+    if (meta_dtype > OSM_META_BF16)
+      return set_diag(diagnostic, "Q4 projection metadata dtype must be F32, F16 or BF16."), std::nullopt;
+    if (group_size == 0U || packed_cols == 0U || out_dim == 0U)
+      return set_diag(diagnostic, "Q4 projection dimensions and group size must be non-zero."), std::nullopt;
+    std::size_t words = 0, groups = 0;
+    if (!mul_ok(out_dim, packed_cols, words) || packed_cols > std::numeric_limits<std::size_t>::max() / 8U ||
+        !mul_ok(out_dim, packed_cols * 8U / group_size, groups))
+      return set_diag(diagnostic, "Q4 shape overflow."), std::nullopt;
+    if (!validate_q4(out_dim, packed_cols, group_size, words, groups, groups, diagnostic)) return std::nullopt;
+    if (packed == nullptr || scales == nullptr || biases == nullptr)
+      return set_diag(diagnostic, "Q4 projection weights, scales and biases must be provided."), std::nullopt;
+    if ((reinterpret_cast<std::uintptr_t>(packed) | reinterpret_cast<std::uintptr_t>(scales) |
+         reinterpret_cast<std::uintptr_t>(biases)) %
+            16U !=
+        0U)
+      return set_diag(diagnostic, "Q4 projection device arrays must be 16-byte aligned."), std::nullopt;
+    auto impl = std::make_unique<Impl>();
+    impl->packed_at = packed;
+    impl->scales_at = scales;
+    impl->biases_at = biases;
+    impl->out_dim = out_dim;
+    impl->packed_cols = packed_cols;
+    impl->group = group_size;
+    impl->meta_dtype = meta_dtype;
+    impl->device = context.device();
+    HipQ4ProjectionWeights w;
+    w.impl_ = std::move(impl);
+    set_diag(diagnostic, "Q4 projection over device arrays.");
+    return w;
+  } catch (const std::exception& e) {
+    set_diag(diagnostic, std::string("Q4 projection exception: ") + e.what());
+    return std::nullopt;
+  }
+}
+
+bool HipQ4ProjectionWeights::valid() const noexcept { return impl_ && impl_->packed_at; }
 std::size_t HipQ4ProjectionWeights::out_dim() const noexcept { return impl_ ? impl_->out_dim : 0; }
 std::size_t HipQ4ProjectionWeights::packed_cols() const noexcept { return impl_ ? impl_->packed_cols : 0; }
 std::size_t HipQ4ProjectionWeights::in_dim() const noexcept { return packed_cols() * 8U; }
 std::size_t HipQ4ProjectionWeights::group_size() const noexcept { return impl_ ? impl_->group : 0; }
 std::uint32_t HipQ4ProjectionWeights::meta_dtype() const noexcept { return impl_ ? impl_->meta_dtype : 0; }
-std::size_t HipQ4ProjectionWeights::packed_size_bytes() const noexcept { return impl_ ? impl_->packed.size() : 0; }
+std::size_t HipQ4ProjectionWeights::packed_size_bytes() const noexcept {
+  return impl_ ? impl_->out_dim * impl_->packed_cols * sizeof(std::uint32_t) : 0;
+}
 std::size_t HipQ4ProjectionWeights::meta_size_bytes() const noexcept {
-  return impl_ ? impl_->scales.size() + impl_->biases.size() : 0;
+  return impl_ ? 2U * impl_->out_dim * (impl_->packed_cols * 8U / impl_->group) * osm_meta_bytes(impl_->meta_dtype) : 0;
 }
 int HipQ4ProjectionWeights::device() const noexcept { return impl_ ? impl_->device : -1; }
 osmd_q4_proj HipQ4ProjectionWeights::view() const noexcept {
   osmd_q4_proj p{};
   if (!impl_) return p;
-  p.packed = impl_->packed.as<const std::uint32_t>();
-  p.scales = impl_->scales.get();
-  p.biases = impl_->biases.get();
+  p.packed = impl_->packed_at;
+  p.scales = impl_->scales_at;
+  p.biases = impl_->biases_at;
   p.out_dim = static_cast<std::uint32_t>(impl_->out_dim);
   p.packed_cols = static_cast<std::uint32_t>(impl_->packed_cols);
   p.group = static_cast<std::uint32_t>(impl_->group);

@@ -114,6 +114,7 @@ class HipComputeContext {
   // until the context ends, so that graphs captured over it stay valid.
   // Returns nullptr (and the HIP error in *rc) when the allocation fails.
   [[nodiscard]] void* shared_workspace(std::size_t bytes, int* rc) noexcept;
+  [[nodiscard]] std::size_t shared_workspace_bytes() const noexcept;
 
  private:
   struct Impl;
@@ -181,6 +182,14 @@ class HipQ4ProjectionWeights {
       HipComputeContext& context, std::span<const std::uint32_t> packed,
       std::size_t out_dim, std::size_t packed_cols, const void* scales,
       const void* biases, std::uint32_t meta_dtype, std::size_t group_size,
+      std::string* diagnostic = nullptr) noexcept;
+
+  // Weights that are on the device already, not copied: the caller keeps the
+  // arrays (16-byte aligned) alive and unchanged while calls that use them run.
+  [[nodiscard]] static std::optional<HipQ4ProjectionWeights> on_device(
+      HipComputeContext& context, const std::uint32_t* packed, std::size_t out_dim,
+      std::size_t packed_cols, const void* scales, const void* biases,
+      std::uint32_t meta_dtype, std::size_t group_size,
       std::string* diagnostic = nullptr) noexcept;
 
   [[nodiscard]] bool valid() const noexcept;
@@ -257,6 +266,34 @@ struct HipQuantizeResult {
 [[nodiscard]] HipValuesResult run_hip_rms_norm(
     HipComputeContext& context, std::span<const float> input, std::size_t rows,
     std::size_t dim, std::span<const float> weight, float eps) noexcept;
+// Routing to experts by a rule, rows grouped by key, and a q4 projection of
+// many tokens with adapters, over device pointers: stream-ordered, no
+// synchronisation (no counterpart in the reference; the C ABI's comments hold
+// the formulas).
+struct HipRouteRule {
+  std::uint32_t expert_count{};
+  std::uint32_t top_k{};
+  std::uint32_t score{};        // OSMD_SCORE_*
+  std::uint32_t groups{1};
+  std::uint32_t top_groups{1};
+  std::uint32_t group_score{1};
+  bool renormalize{true};
+  float scale{1.0F};
+};
+[[nodiscard]] bool check_route_rule(const HipRouteRule& rule, std::string* diagnostic) noexcept;
+[[nodiscard]] HipDispatchResult run_hip_route_experts(
+    HipComputeContext& context, const HipRouteRule& rule, const void* logits,
+    std::uint32_t logits_dtype, std::size_t logits_stride, const float* bias,
+    std::uint32_t tokens, std::uint32_t* ids, float* weights, float* mass) noexcept;
+[[nodiscard]] HipDispatchResult run_hip_group_rows(
+    HipComputeContext& context, const std::int32_t* keys, std::uint32_t rows,
+    std::uint32_t buckets, std::uint32_t* offsets, std::uint32_t* order) noexcept;
+// adapters.count == 0: the projection alone. Strides 0: dense rows.
+[[nodiscard]] HipDispatchResult run_hip_q4_project(
+    HipComputeContext& context, const HipQ4ProjectionWeights& weights, const void* x,
+    std::uint32_t x_dtype, std::size_t x_stride, void* y, std::uint32_t y_dtype,
+    std::size_t y_stride, std::uint32_t tokens, const osmd_adapters& adapters,
+    const std::int32_t* adapter_ids) noexcept;
 // Nibble unpack (integer-exact check of the packed layout): out[8*w + j] is
 // nibble j (low first) of word w.
 [[nodiscard]] bool run_hip_unpack_nibbles(HipComputeContext& context,
@@ -836,6 +873,10 @@ class HipMoeLayer {
                                          std::uint32_t tokens, const std::uint8_t* const* expert_table,
                                          bool sublayer, const char** diagnostic) noexcept;
   [[nodiscard]] std::uint32_t static_tokens_capacity() const noexcept;
+  // Selection by a rule instead of the softmax top-k (nullptr: that again),
+  // on every path; bias: expert_count values or none. Waits for the stream.
+  [[nodiscard]] bool set_routing(HipComputeContext& context, const HipRouteRule* rule, std::span<const float> bias,
+                                 std::string* diagnostic = nullptr) noexcept;
   // False (path unchanged) for a value that names no path.
   bool set_path(HipMoePath path, std::string* diagnostic = nullptr) noexcept;
   [[nodiscard]] HipMoePath path() const noexcept;

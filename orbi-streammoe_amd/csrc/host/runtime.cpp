@@ -109,6 +109,8 @@ void* HipComputeContext::shared_workspace(std::size_t bytes, int* rc) noexcept {
   }
 }
 
+std::size_t HipComputeContext::shared_workspace_bytes() const noexcept { return impl_ ? impl_->workspace.size() : 0; }
+
 HipComputeContext::HipComputeContext() = default;
 HipComputeContext::~HipComputeContext() = default;
 HipComputeContext::HipComputeContext(HipComputeContext&&) noexcept = default;

@@ -25,6 +25,7 @@ LIB_PATH = os.path.join(HERE, "libosm_hip.so")
 OSM_OK, OSM_E_INVALID, OSM_E_RUNTIME, OSM_E_DEVICE = 0, 1, 2, 3
 PATH_AUTO, PATH_PER_TOKEN, PATH_GROUPED = 0, 1, 2
 F32, F16, BF16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1  # RouteRule.score
 AFFINE_Q8 = 3  # router / shared-gate dtype: MLX affine 8-bit (osm_affine_q8_c)
 
 
@@ -60,6 +61,27 @@ class MoeOutputs(ctypes.Structure):
         ("shared_gate", c_void_p),
         ("logits", c_void_p),
     ]
+
+
+class RouteRule(ctypes.Structure):
+    """How tokens pick experts (osm_route_rule): route_experts, MoeLayer.set_routing."""
+
+    _fields_ = [(n, c_uint32) for n in ("expert_count", "top_k", "score", "groups", "top_groups", "group_score", "renormalize")] + [
+        ("scale", c_float)]
+
+    def __init__(self, expert_count, top_k, score=SCORE_SOFTMAX, groups=1, top_groups=1, group_score=1, renormalize=True, scale=1.0):
+        super().__init__(expert_count, top_k, score, groups, top_groups, group_score, int(renormalize), scale)
+
+
+class Adapters(ctypes.Structure):
+    """Low-rank adapters in device memory (osm_adapters): a [count, max_rank, in_dim], b [count, out_dim, max_rank],
+    optional scales [count] fp32 and ranks [count] uint32. The caller keeps the arrays alive."""
+
+    _fields_ = [("a", c_void_p), ("b", c_void_p), ("scales", c_void_p), ("ranks", c_void_p), ("count", c_uint32),
+                ("max_rank", c_uint32), ("dtype", c_uint32)]
+
+    def __init__(self, a_ptr, b_ptr, count, max_rank, dtype=BF16, scales=None, ranks=None):
+        super().__init__(a_ptr, b_ptr, scales, ranks, count, max_rank, dtype)
 
 
 class HostCacheStats(ctypes.Structure):
@@ -110,7 +132,12 @@ _PROTOTYPES = {
     "osm_q4_quantize": (c_int, [_H, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p, POINTER(c_float), POINTER(ctypes.c_double)]),
     "osm_q4_gemv_buffers": (c_int, [_H, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_size_t, c_size_t, _H, _H]),
     "osm_q4_projection_create": (c_int, [_H, c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_uint32, c_size_t, POINTER(_H)]),
+    "osm_q4_projection_on_device": (c_int, [_H, c_void_p, c_size_t, c_size_t, c_void_p, c_void_p, c_uint32, c_size_t, POINTER(_H)]),
     "osm_q4_projection_destroy": (None, [_H]),
+    "osm_route_experts": (c_int, [_H, POINTER(RouteRule), c_void_p, c_uint32, c_size_t, c_void_p, c_uint32, c_void_p, c_void_p, c_void_p]),
+    "osm_group_rows": (c_int, [_H, c_void_p, c_uint32, c_uint32, c_void_p, c_void_p]),
+    "osm_q4_project": (c_int, [_H, _H, c_void_p, c_uint32, c_size_t, c_void_p, c_uint32, c_size_t, c_uint32, POINTER(Adapters), c_void_p]),
+    "osm_moe_layer_set_routing": (c_int, [_H, _H, POINTER(RouteRule), c_void_p]),
     "osm_q4_gemv_preloaded": (c_int, [_H, _H, _H, _H]),
     "osm_swiglu_buffers": (c_int, [_H, _H, _H, _H]),
     "osm_weighted_accumulate": (c_int, [_H, _H, c_float, _H]),
@@ -544,6 +571,36 @@ class Q4ProjectionWeights(_Handle):
         super().__init__(h)
         ctx._adopt(self)
 
+    @classmethod
+    def on_device(cls, ctx, packed_ptr, out_dim, packed_cols, scales_ptr, biases_ptr, group_size, meta_dtype=F32):
+        """Over arrays that are on the device already (osm_q4_projection_on_device); the caller keeps them alive."""
+        h = c_void_p()
+        check(load().osm_q4_projection_on_device(ctx.h, packed_ptr, out_dim, packed_cols, scales_ptr, biases_ptr, meta_dtype,
+                                                 group_size, ctypes.byref(h)))
+        self = cls.__new__(cls)
+        _Handle.__init__(self, h)
+        ctx._adopt(self)
+        return self
+
+
+def route_experts(ctx, rule: RouteRule, logits_ptr, logits_dtype, tokens, ids_ptr, weights_ptr, bias_ptr=None, mass_ptr=None,
+                  logits_stride=0):
+    """Device logits [tokens, E] to picks ids / weights [tokens, k] by the rule (osm_route_experts)."""
+    check(load().osm_route_experts(ctx.h, ctypes.byref(rule), logits_ptr, logits_dtype, logits_stride, bias_ptr, tokens, ids_ptr,
+                                   weights_ptr, mass_ptr))
+
+
+def group_rows(ctx, keys_ptr, rows, buckets, offsets_ptr, order_ptr):
+    """Device int32 keys [rows] to offsets [buckets + 1] and order [rows], stable (osm_group_rows)."""
+    check(load().osm_group_rows(ctx.h, keys_ptr, rows, buckets, offsets_ptr, order_ptr))
+
+
+def q4_project(ctx, weights: "Q4ProjectionWeights", x_ptr, y_ptr, tokens, x_dtype=F32, y_dtype=F32, x_stride=0, y_stride=0,
+               adapters: Adapters = None, adapter_ids_ptr=None):
+    """Device x [tokens, in_dim] to y [tokens, out_dim], each token with its own adapter (osm_q4_project)."""
+    check(load().osm_q4_project(ctx.h, weights.h, x_ptr, x_dtype, x_stride, y_ptr, y_dtype, y_stride, tokens,
+                                ctypes.byref(adapters) if adapters is not None else None, adapter_ids_ptr))
+
 
 def run_q4_gemv_preloaded(ctx, weights: Q4ProjectionWeights, x: FloatBuffer, y: FloatBuffer):
     check(load().osm_q4_gemv_preloaded(ctx.h, weights.h, x.h, y.h))
@@ -734,6 +791,14 @@ class MoeLayer(_Handle):
     @property
     def static_tokens_capacity(self) -> int:
         return int(load().osm_moe_layer_static_tokens_capacity(self.h))
+
+    def set_routing(self, rule: RouteRule = None, bias=None):
+        """Selects by a rule (with a host bias [E] or None) from now on; None: softmax top-k again."""
+        b = _c(bias, np.float32) if bias is not None else None
+        if b is not None and b.size != self.E:
+            raise ValueError("the bias has one value per expert")
+        check(load().osm_moe_layer_set_routing(self.ctx.h, self.h, ctypes.byref(rule) if rule is not None else None,
+                                               _p(b) if b is not None else None))
 
     def set_path(self, path):
         """PATH_AUTO, PATH_PER_TOKEN or PATH_GROUPED."""

@@ -1,0 +1,56 @@
+"""Rows grouped by key (osm_group_rows) against numpy's stable sort."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import osm_hip
+
+pytestmark = pytest.mark.gpu
+
+
+def group(ctx, keys, buckets):
+    n = keys.size
+    k, off, order = ctx.alloc(4 * n + 64), ctx.alloc(4 * (buckets + 1) + 64), ctx.alloc(4 * n + 64)
+    k.upload(np.concatenate([keys, np.zeros(16, np.int32)]))  # rows behind the last: key 0, not counted
+    for a in (off, order):
+        a.upload(np.full(a.nbytes // 4, 0xABABABAB, np.uint32))
+    osm_hip.group_rows(ctx, k.ptr, n, buckets, off.ptr, order.ptr)
+    ctx.synchronize()
+    o, r = off.download(np.uint32, off.nbytes // 4), order.download(np.uint32, order.nbytes // 4)
+    assert np.all(o[buckets + 1:] == 0xABABABAB) and np.all(r[n:] == 0xABABABAB)
+    return o[:buckets + 1], r[:n]
+
+
+def expected(keys, buckets):
+    b = np.where((keys >= 0) & (keys < buckets), keys, buckets)
+    counts = np.bincount(b, minlength=buckets + 1)
+    return np.cumsum(counts) - counts, np.argsort(b, kind="stable")
+
+
+@pytest.mark.parametrize("n", [0, 1, 63, 64, 65, 1000, 1025, 4097, 81920, 300007])
+@pytest.mark.parametrize("buckets", [1, 2, 7, 255, 256, 512, 1000, 65535])
+def test_matches_stable_sort(ctx, n, buckets):
+    rng = np.random.default_rng(n + buckets)
+    print(f"[group] n={n} buckets={buckets}", flush=True)
+    uniform = rng.integers(0, buckets, n)
+    skewed = np.minimum(rng.geometric(0.3, n) - 1, buckets - 1)
+    keys = {"uniform": uniform, "outside": np.where(rng.random(n) < 0.3, rng.choice([-1, buckets, -(2**31), 2**31 - 1], n), uniform),
+            "skewed": skewed, "one": np.full(n, buckets - 1), "sorted": np.sort(uniform), "none": np.full(n, -5)}
+    for name, k in keys.items():
+        k = k.astype(np.int32)
+        offsets, order = group(ctx, k, buckets)
+        ref_offsets, ref_order = expected(k, buckets)
+        assert np.array_equal(offsets, ref_offsets), name
+        assert np.array_equal(order, ref_order), name
+
+
+def test_refused(ctx):
+    a = ctx.alloc(256)
+    odd = ctypes.c_void_p(a.ptr.value + 2)
+    for args in ((a.ptr, 4, 0, a.ptr, a.ptr), (a.ptr, 4, 65536, a.ptr, a.ptr), (None, 4, 2, a.ptr, a.ptr), (a.ptr, 4, 2, None, a.ptr),
+                 (a.ptr, 4, 2, a.ptr, None), (odd, 4, 2, a.ptr, a.ptr), (a.ptr, 2**31, 2, a.ptr, a.ptr)):
+        with pytest.raises(osm_hip.OsmError) as e:
+            osm_hip.group_rows(ctx, *args)
+        assert e.value.status == osm_hip.OSM_E_INVALID and e.value.diagnostic
