@@ -110,8 +110,12 @@ struct PrepareParams {
 };
 
 // TPT threads per row, 256 / TPT rows per workgroup.
-template <int XT, int R, int GW, int TPT>
-__device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t block) {
+struct ManyPrepared;
+template <int TERMS>
+__device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v);
+
+template <int XT, int R, int GW, int TPT, bool MANY = false>
+__device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t block, const ManyPrepared* many = nullptr) {
   constexpr int NT = XT == OSM_META_F32 ? 2 : 1;
   constexpr uint32_t GWS = GW * kSlots<R>;  // words of a sub-group
   __shared__ float red[256 / kWave];
@@ -167,7 +171,15 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
     *reinterpret_cast<f16x8*>(f) = hi;
     if constexpr (NT == 2) *reinterpret_cast<f16x8*>(f + kWave * 8u) = lo;
     sum = row_sum<GWS < 16 ? GWS : 16>(sum);
-    if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
+    if constexpr (MANY) {
+      if (iw == 0) {
+        store_sum<3>(*many, tile, sub, row % R, sum * 0x1p-24f);
+        if (sub + 1u == subs)
+          for (uint32_t z = subs; z % 16u != 0u; ++z) store_sum<3>(*many, tile, z, row % R, 0.0f);
+      }
+    } else {
+      if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
+    }
   }
 }
 
@@ -215,8 +227,8 @@ __global__ __launch_bounds__(256) void prepare_few_kernel(PrepareParams p, Shrin
 }
 
 // ---- few tokens ------------------------------------------------------------------
-// A workgroup owns R rows of W and all (at most MT * R) tokens; its wavefronts
-// split the columns and their sums are added in LDS in wavefront order. The
+// A workgroup owns R rows of W and R tokens; its wavefronts split the columns
+// and their sums are added in LDS in wavefront order. The
 // lanes of an instruction's D columns are rows of W, so a lane needs one
 // scale and bias per sub-group.
 template <int R>
@@ -248,22 +260,6 @@ __device__ __forceinline__ f16x8 nibble_operand(uint32_t w) {
 }
 __device__ __forceinline__ f16x8 load_frag(const _Float16* p) { return __builtin_bit_cast(f16x8, ldg<u32x4>(p)); }
 
-template <int GW>
-__device__ __forceinline__ void load_words(const uint32_t* p, uint32_t (&w)[GW]) {
-  if constexpr (GW == 1) {
-    w[0] = ldg<uint32_t>(p);
-  } else if constexpr (GW == 2) {
-    const uint2 v = ldg8(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < GW / 4; ++i) {
-      const uint4 v = ldg16(p + 4 * i);
-      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-    }
-  }
-}
-
 struct ProjectParams {
   osmd_q4_proj w;
   uint32_t groups, per_group;  // groups of a row, sub-groups of a group
@@ -274,7 +270,7 @@ struct ProjectParams {
   osmd_adapters ad;
   const int32_t* ids;
   uint32_t b_wide;
-  const uint32_t* order;
+  uint32_t stage_subs, stage_log2;  // few tokens: sub-groups of a stage, log2 of its chunks rounded up
 };
 
 __device__ __forceinline__ float adapter_element(const osmd_adapters& ad, size_t o) {
@@ -283,105 +279,703 @@ __device__ __forceinline__ float adapter_element(const osmd_adapters& ad, size_t
                                      : meta_at<OSM_META_F16>(ad.b, o);
 }
 
+// Columns of B taken ahead of their use (16-bit adapters, rows of whole
+// 16-byte pieces): up to 16.
+struct ExpandAhead {
+  uint32_t a, rank;
+  uint4 b[2];
+};
+__device__ __forceinline__ void expand_ahead(const ProjectParams& p, uint32_t t, uint32_t n, ExpandAhead& x) {
+  x.a = 0;
+  x.rank = token_rank(p.ad, p.ids, t, x.a);
+  if (p.b_wide && p.ad.dtype != OSM_META_F32 && x.rank != 0u) {
+    const uint16_t* b = static_cast<const uint16_t*>(p.ad.b) + (static_cast<size_t>(x.a) * p.w.out_dim + n) * p.ad.max_rank;
+    x.b[0] = ldg16(b);
+    x.b[1] = ldg16(b + (p.ad.max_rank > 8u ? 8u : 0u));
+  }
+}
+
+// s + the first `count` (at most 8) of b . v.
+template <typename B>
+__device__ __forceinline__ float dot8(const B& b, const float* v, uint32_t count, float s) {
+  const float4 lo = *reinterpret_cast<const float4*>(v), hi = *reinterpret_cast<const float4*>(v + 4);
+  const float c[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s = static_cast<uint32_t>(k) < count ? fmaf(b[k], c[k], s) : s;
+  return s;
+}
+
 // (B_a v_t)_n for one token and row.
-__device__ __forceinline__ float expand_one(const ProjectParams& p, uint32_t t, uint32_t n) {
-  uint32_t a = 0;
-  const uint32_t rank = token_rank(p.ad, p.ids, t, a);
-  const size_t o = (static_cast<size_t>(a) * p.w.out_dim + n) * p.ad.max_rank;
+__device__ __forceinline__ float expand_one(const ProjectParams& p, uint32_t t, uint32_t n, const ExpandAhead& x) {
+  if (x.rank == 0u) return 0.0f;
+  const size_t o = (static_cast<size_t>(x.a) * p.w.out_dim + n) * p.ad.max_rank;
   const float* v = p.in.v + static_cast<size_t>(t) * p.in.vr;
   float s = 0.0f;
   uint32_t j = 0;
-  if (p.b_wide) {
-    for (; j + 8u <= rank; j += 8u) {
-      float b[8], c[8];
-      if (p.ad.dtype == OSM_META_BF16)
-        load8<OSM_META_BF16>(p.ad.b, o + j, true, b);
-      else if (p.ad.dtype == OSM_META_F16)
-        load8<OSM_META_F16>(p.ad.b, o + j, true, b);
-      else
-        load8<OSM_META_F32>(p.ad.b, o + j, true, b);
-      load8<OSM_META_F32>(v, j, true, c);
+  if (p.b_wide && p.ad.dtype != OSM_META_F32) {
+    const bool bf = p.ad.dtype == OSM_META_BF16;
+    for (; j < x.rank; j += 8u) {
+      const uint4 q = j == 0u ? x.b[0] : j == 8u ? x.b[1] : ldg16(static_cast<const uint16_t*>(p.ad.b) + o + j);
+      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+      float b[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s = fmaf(b[k], c[k], s);
+      for (int i = 0; i < 4; ++i) {
+        b[2 * i] = bf ? bf16_to_f32(u[i] & 0xFFFFu) : f16_to_f32(u[i] & 0xFFFFu);
+        b[2 * i + 1] = bf ? __uint_as_float(u[i] & 0xFFFF0000u) : f16_to_f32(u[i] >> 16);
+      }
+      s = dot8(b, v + j, x.rank - j, s);
     }
+    return s;
   }
-  for (; j < rank; ++j) s = fmaf(adapter_element(p.ad, o + j), v[j], s);
+  for (; j < x.rank; ++j) s = fmaf(adapter_element(p.ad, o + j), v[j], s);
   return s;
 }
 
 constexpr int kFewWaves = 8;
+constexpr int kWaitVmcnt0 = 0x0F70;  // s_waitcnt operand: vector memory counter 0, the others at their maximum
 
-template <int R, int NT, int MT, int GW, int META>
-__global__ __launch_bounds__(kFewWaves* kWave) void project_few_kernel(ProjectParams p) {
+// 16 bytes per lane from global memory straight into LDS, lane l's at
+// dst + 16 l (dst wave-uniform).
+__device__ __forceinline__ void load_lds16(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+}
+
+// A stage is what a workgroup holds in LDS at a time: its R rows' words of
+// up to 4096 (R = 16) or 2048 columns, which are contiguous in memory row by
+// row, so every load moves whole lines (read by the lanes in operand order
+// they took several times as long, a wavefront touching 16 or 32 lines an
+// instruction); with them the scales and biases widened to fp32 and the
+// tokens' group sums. Chunk c of 16 bytes of row r sits at (r << lc) + (c ^ (r
+// & 15)), which spreads the rows' equal chunks over the banks.
+template <int R, int NT, int GW, int META>
+__global__ __launch_bounds__(kFewWaves* kWave, 4) void project_few_kernel(ProjectParams p) {
   typedef typename Tile<R>::acc acc_t;
   constexpr int A = kAcc<R>;
   constexpr uint32_t GWS = GW * kSlots<R>;
-  constexpr int U = 4;  // sub-groups in flight
-  __shared__ float part[kFewWaves][MT][A][kWave];
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  constexpr uint32_t kChunks = 2048u / R;          // of a row in a stage
+  constexpr uint32_t kSubs = kChunks * 4u / GWS;   // sub-groups in a stage
+  constexpr int P = (R * R + kFewWaves * kWave - 1) / (kFewWaves * kWave);  // outputs of a thread
+  __shared__ __attribute__((aligned(16))) union {
+    uint4 w[R * kChunks];
+    float part[kFewWaves][A][kWave];
+  } lds;
+  __shared__ float scale[kSubs][R + 1], bias[kSubs][R + 1];
+  __shared__ __attribute__((aligned(16))) float sums[kSubs * R];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const uint32_t N = p.w.out_dim, words = p.w.packed_cols, subs = words / GWS, steps = subs * GW;
-  const uint32_t n0 = blockIdx.x * R;
-  const uint32_t n = n0 + lane % R < N ? n0 + lane % R : N - 1u;
-  const uint32_t s0 = subs * wave / kFewWaves, s1 = subs * (wave + 1u) / kFewWaves;
-  const uint32_t* wrow = p.w.packed + static_cast<size_t>(n) * words + lane / R * GW;
-  const size_t mrow = static_cast<size_t>(n) * p.groups;
-  const _Float16* frag = p.in.frag + lane * 8u;
-  acc_t total[MT];
+  const uint32_t n0 = blockIdx.x * R, tile = blockIdx.y, row = lane % R, slot = lane / R;
+  const uint32_t lc = p.stage_log2, swizzle = (1u << lc) - 1u < 15u ? (1u << lc) - 1u : 15u;
+  const _Float16* frag = p.in.frag + static_cast<size_t>(tile) * steps * NT * kWave * 8u + lane * 8u;
+  const float* tile_sums = p.in.sums + static_cast<size_t>(tile) * subs * R;
+  acc_t total;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < A; ++i) total[i] = 0.0f;
+  ExpandAhead ahead[P];
 #pragma unroll
-    for (int i = 0; i < A; ++i) total[m][i] = 0.0f;
-  for (uint32_t s = s0; s < s1; s += U) {
-    uint32_t w[U][GW];
-    uint32_t sb[U], bb[U];
+  for (int o = 0; o < P; ++o) ahead[o].rank = 0u;
+  for (uint32_t S0 = 0; S0 < subs; S0 += p.stage_subs) {
+    const uint32_t S = subs - S0 < p.stage_subs ? subs - S0 : p.stage_subs;
+    if (S0 != 0u) __syncthreads();  // the stage before is read
+    const uint32_t chunks = S * GWS / 4u;
+    for (uint32_t i0 = wave * kWave; i0 < R << lc; i0 += kFewWaves * kWave) {
+      const uint32_t i = i0 + lane, r = i >> lc, c = (i & ((1u << lc) - 1u)) ^ (r & swizzle);
+      const size_t n = n0 + r < N ? n0 + r : N - 1u;
+      if (i < R << lc) load_lds16(p.w.packed + n * words + S0 * GWS + 4u * (c < chunks ? c : chunks - 1u), &lds.w[i0]);
+    }
+    for (uint32_t i0 = wave * kWave; i0 < S * R / 4u; i0 += kFewWaves * kWave)
+      if (i0 + lane < S * R / 4u) load_lds16(tile_sums + S0 * R + 4u * (i0 + lane), sums + 4u * i0);
+    for (uint32_t i = tid; i < R * S; i += kFewWaves * kWave) {
+      const uint32_t r = i / S, s = i % S;
+      const size_t o = static_cast<size_t>(n0 + r < N ? n0 + r : N - 1u) * p.groups + (S0 + s) / p.per_group;
+      scale[s][r] = meta_at<META>(p.w.scales, o);
+      bias[s][r] = meta_at<META>(p.w.biases, o);
+    }
+    const uint32_t s0 = S * wave / kFewWaves, s1 = S * (wave + 1u) / kFewWaves;
+    // The next sub-group's operands are loaded while one computes; not in the
+    // widest case, where two workgroups' registers (128 a lane) hold one.
+    constexpr bool kNext = R == 16 || GW * NT < 8;
+    f16x8 x[kNext ? 2 : 1][GW * NT];
+    auto load = [&](f16x8 (&v)[GW * NT], uint32_t s) {
+      const uint32_t c = S0 + (s < s1 ? s : s0 < s1 ? s1 - 1u : 0u);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t c = s + u < s1 ? s + u : s1 - 1u;
-      load_words<GW>(wrow + c * GWS, w[u]);
-      sb[u] = meta_bits<META>(p.w.scales, mrow + c / p.per_group);
-      bb[u] = meta_bits<META>(p.w.biases, mrow + c / p.per_group);
+      for (int k = 0; k < GW * NT; ++k) v[k] = load_frag(frag + (static_cast<size_t>(c) * GW * NT + k) * kWave * 8u);
+    };
+    load(x[0], s0);
+    if (S0 == 0u && p.ad.count) {
+#pragma unroll
+      for (int o = 0; o < P; ++o) {
+        const uint32_t i = tid + o * kFewWaves * kWave, t = tile * R + i / R, nn = n0 + i % R;
+        if (i < R * R && t < p.tokens && nn < N) expand_ahead(p, t, nn, ahead[o]);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    __syncthreads();
+    auto compute = [&](const f16x8 (&v)[GW * NT], uint32_t s) {
+      const uint32_t word = s * GWS + slot * GW;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(&lds.w[(row << lc) + ((word / 4u) ^ (row & swizzle))]) + word % 4u;
+      uint32_t w[GW];
+      if constexpr (GW == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+      } else if constexpr (GW == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(q);
+        w[0] = u.x, w[1] = u.y;
+      } else {
+        w[0] = *q;
+      }
+      const float sc = scale[s][row], bc = bias[s][row];
+      acc_t d;
+#pragma unroll
+      for (int i = 0; i < A; ++i) d[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < GW; ++k) {
+        const f16x8 b = nibble_operand(w[k]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) d = Tile<R>::mfma(v[k * NT + t], b, d);
+      }
+#pragma unroll
+      for (int i = 0; i < A / 4; ++i) {
+        const float4 xs = *reinterpret_cast<const float4*>(sums + s * R + Tile<R>::row(lane, 4 * i));
+        total[4 * i] = fmaf(sc, d[4 * i], fmaf(bc, xs.x, total[4 * i]));
+        total[4 * i + 1] = fmaf(sc, d[4 * i + 1], fmaf(bc, xs.y, total[4 * i + 1]));
+        total[4 * i + 2] = fmaf(sc, d[4 * i + 2], fmaf(bc, xs.z, total[4 * i + 2]));
+        total[4 * i + 3] = fmaf(sc, d[4 * i + 3], fmaf(bc, xs.w, total[4 * i + 3]));
+      }
+    };
+    if constexpr (kNext) {
+      for (uint32_t s = s0; s < s1; s += 2u) {
+        load(x[1], s + 1u);
+        compute(x[0], s);
+        load(x[0], s + 2u);
+        if (s + 1u < s1) compute(x[1], s + 1u);
+      }
+    } else {
+      for (uint32_t s = s0; s < s1; ++s) {
+        compute(x[0], s);
+        load(x[0], s + 1u);
+      }
+    }
+  }
+  // The adapters' part of each output, while other wavefronts still sum.
+  float e[P] = {};
+  if (p.ad.count) {
+#pragma unroll
+    for (int o = 0; o < P; ++o) {
+      const uint32_t i = tid + o * kFewWaves * kWave;
+      e[o] = expand_one(p, tile * R + i / R, n0 + i % R, ahead[o]);
+    }
+  }
+  __syncthreads();  // the words are read; their place holds the sums
+#pragma unroll
+  for (int i = 0; i < A; ++i) lds.part[wave][i][lane] = total[i];
+  __syncthreads();
+#pragma unroll
+  for (int o = 0; o < P; ++o) {
+    const uint32_t i = tid + o * kFewWaves * kWave, tr = i / R, t = tile * R + tr, nn = n0 + i % R;
+    if (i >= R * R || t >= p.tokens || nn >= N) continue;
+    const uint32_t r = R == 16 ? tr % 4u : tr / 8u * 4u + tr % 4u;
+    const uint32_t l = (R == 16 ? tr / 4u : tr / 4u % 2u) * R + i % R;
+    float y = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kFewWaves; ++k) y += lds.part[k][r][l];
+    store_out(p.y, p.y_dtype, t * p.y_stride + nn, ldexpf(y, p.in.exps[t]) + e[o]);
+  }
+}
+
+// ---- one to four tokens ----------------------------------------------------------
+// A wavefront takes kVecRows rows of W; a lane holds 32 consecutive columns of
+// each token in registers (a chunk, within one quantisation group) and the
+// chunk's sum for the bias. No preparation: one launch, after the shrink.
+constexpr int kVecWaves = 4;
+
+template <int XT>
+__device__ __forceinline__ void load32(const void* x, size_t o, bool wide, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float u[8];
+    load8<XT>(x, o + 8u * i, wide, u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[8 * i + k] = u[k];
+  }
+}
+
+struct VecParams {
+  ProjectParams p;
+  const void* x;
+  size_t stride;
+  uint32_t wide;
+};
+
+template <int META, int XT, int TV, int ROWS>
+__global__ __launch_bounds__(kVecWaves* kWave) void project_vec_kernel(VecParams vp) {
+  const ProjectParams& p = vp.p;
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const uint32_t N = p.w.out_dim, words = p.w.packed_cols, chunks = words / 4u, G = p.w.group;
+  const uint32_t n0 = (blockIdx.x * kVecWaves + wave) * ROWS, t0 = blockIdx.y * TV;
+  if (n0 >= N) return;
+  float acc[ROWS][TV] = {};
+  for (uint32_t c = lane; c < chunks; c += kWave) {
+    uint4 q[ROWS];
+    uint32_t sb[ROWS], bb[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const size_t n = n0 + r < N ? n0 + r : N - 1u;
+      q[r] = ldg16(p.w.packed + n * words + 4u * c);
+      sb[r] = meta_bits<META>(p.w.scales, n * p.groups + 32u * c / G);
+      bb[r] = meta_bits<META>(p.w.biases, n * p.groups + 32u * c / G);
+    }
+    float x[TV][32], sum[TV];
+#pragma unroll
+    for (int t = 0; t < TV; ++t) {
+      load32<XT>(vp.x, (t0 + t < p.tokens ? t0 + t : t0) * vp.stride + 32u * c, vp.wide, x[t]);
+      sum[t] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) sum[t] += x[t][k];
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s + u >= s1) break;
-      const uint32_t c = s + u;
-      f16x8 q[GW];
+    for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-      for (int g = 0; g < GW; ++g) q[g] = nibble_operand(w[u][g]);
-      const float sc = meta_widen<META>(sb[u]), bc = meta_widen<META>(bb[u]);
+      for (int t = 0; t < TV; ++t)
+        acc[r][t] = fmaf(meta_widen<META>(sb[r]), nib_dot32(q[r], x[t]), fmaf(meta_widen<META>(bb[r]), sum[t], acc[r][t]));
+  }
+  // The adapters' columns, one a lane, join the lanes' sums.
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        acc_t d;
+  for (int t = 0; t < TV; ++t) {
+    uint32_t a = 0;
+    const uint32_t rank = t0 + t < p.tokens ? token_rank(p.ad, p.ids, t0 + t, a) : 0u;
+    for (uint32_t j = lane; j < rank; j += kWave) {
+      const float v = p.in.v[static_cast<size_t>(t0 + t) * p.in.vr + j];
 #pragma unroll
-        for (int i = 0; i < A; ++i) d[i] = 0.0f;
-        const _Float16* f = frag + (static_cast<size_t>(m) * steps + c * GW) * NT * kWave * 8u;
-#pragma unroll
-        for (int g = 0; g < GW; ++g)
-#pragma unroll
-          for (int k = 0; k < NT; ++k) d = Tile<R>::mfma(load_frag(f + (g * NT + k) * kWave * 8u), q[g], d);
-        const float* xs = p.in.sums + (static_cast<size_t>(m) * subs + c) * R;
-#pragma unroll
-        for (int i = 0; i < A; ++i)
-          total[m][i] = fmaf(sc, d[i], fmaf(bc, xs[Tile<R>::row(lane, i)], total[m][i]));
+      for (int r = 0; r < ROWS; ++r) {
+        const size_t n = n0 + r < N ? n0 + r : N - 1u;
+        acc[r][t] = fmaf(adapter_element(p.ad, (a * static_cast<size_t>(N) + n) * p.ad.max_rank + j), v, acc[r][t]);
       }
     }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int i = 0; i < A; ++i) part[wave][m][i][lane] = total[m][i];
+    for (int t = 0; t < TV; ++t) {
+      const float y = wave_sum(acc[r][t]);
+      if (lane == 0 && n0 + r < N && t0 + t < p.tokens) store_out(p.y, p.y_dtype, (t0 + t) * p.y_stride + n0 + r, y);
+    }
+}
+
+// ---- many tokens -------------------------------------------------------------------
+// Tiles of 32 x 32 outputs, W unpacked in registers and used for MT tiles of
+// tokens; the tokens' fragments and the packed words are staged through LDS,
+// the next stage's on their way in registers while one computes. Per output
+// and sub-group of 64 columns that is 64 products on the matrix cores against
+// one FMA (the scale) and 64 / (32 MT) unpacked nibbles on the vector units;
+// the biases, a product of [tokens, sub-groups] by [sub-groups, rows], are on
+// the matrix cores too. Their factors are split into bf16 terms (the sums into
+// three; a bias into one, two or three by its type), products below 2^-24 of
+// the whole left out. Before the main launch one prepares x (as above), the
+// scales transposed to [sub-group][row] and the biases as operands.
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <int AT>
+constexpr int kTerms = AT == OSM_META_BF16 ? 1 : AT == OSM_META_F16 ? 2 : 3;  // exact in that many bf16 terms
+
+// v = t[0] + t[1] + ..., each the bf16 nearest to what is left.
+template <int NT>
+__device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[NT]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    float left = v[k];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      t[i][k] = static_cast<__bf16>(left);
+      if (i + 1 < NT) left -= static_cast<float>(t[i][k]);
+    }
+  }
+}
+
+__device__ __forceinline__ f32x16 mfma_bf16(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// c + a b, terms i and j with i + j < 3.
+template <int NA, int NB, typename C>
+__device__ __forceinline__ C mfma_terms(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], C c) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j < 3) c = mfma_bf16(a[i], b[j], c);
+  return c;
+}
+
+constexpr int kSumTerms = 3;
+
+struct ManyPrepared {
+  __bf16* sum_frag;   // [tile][16 sub-groups][term][64][8]
+  float* scales;      // [sub-group][row of W]
+  __bf16* bias_frag;  // [32 rows][16 sub-groups][term][64][8]
+  uint32_t kgs;       // runs of 16 sub-groups
+};
+
+template <int TERMS>
+__device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v) {
+  const uint32_t lane = sub % 16u / 8u * 32u + row;
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    const __bf16 b = static_cast<__bf16>(v);
+    m.sum_frag[(((static_cast<size_t>(tile) * m.kgs + sub / 16u) * TERMS + t) * kWave + lane) * 8u + sub % 8u] = b;
+    v -= static_cast<float>(b);
+  }
+}
+
+// Scales and biases of W for sub-groups of which `per_group` make a group: a
+// workgroup takes 16 sub-groups of 32 rows; what lies past the last is zero.
+template <int META>
+__device__ __forceinline__ void prepare_meta(const osmd_q4_proj& w, uint32_t groups, uint32_t per_group, uint32_t subs,
+                                             const ManyPrepared& out, uint32_t block) {
+  constexpr int NT = kTerms<META>;
+  const uint32_t nb = block / out.kgs, kg = block % out.kgs;
+  for (uint32_t i = threadIdx.x; i < 512u; i += 256u) {
+    const uint32_t r = i % 32u, s = i / 32u, n = nb * 32u + r, sub = kg * 16u + s;
+    const bool in = n < w.out_dim && sub < subs;
+    const size_t o = static_cast<size_t>(in ? n : 0u) * groups + (in ? sub / per_group : 0u);
+    if (in) out.scales[static_cast<size_t>(sub) * w.out_dim + n] = meta_at<META>(w.scales, o);
+    float left = in ? meta_at<META>(w.biases, o) : 0.0f;
+    const uint32_t lane = s / 8u * 32u + r;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const __bf16 b = static_cast<__bf16>(left);
+      out.bias_frag[(((static_cast<size_t>(nb) * out.kgs + kg) * NT + t) * kWave + lane) * 8u + s % 8u] = b;
+      left -= static_cast<float>(b);
+    }
+  }
+}
+
+struct PrepareManyParams {
+  PrepareParams x;
+  ManyPrepared many;
+  osmd_q4_proj w;
+  uint32_t groups, per_group, subs, x_blocks;
+};
+
+template <int XT, int GW, int META>
+__global__ __launch_bounds__(256) void prepare_many_kernel(PrepareManyParams p) {
+  if (blockIdx.x < p.x_blocks)
+    prepare_rows<XT, 32, GW, 32, true>(p.x, blockIdx.x, &p.many);
+  else
+    prepare_meta<META>(p.w, p.groups, p.per_group, p.subs, p.many, blockIdx.x - p.x_blocks);
+}
+
+// v of tiles of 16 tokens (in `order`): x and A_a split into bf16 terms, the
+// wavefronts taking the columns in turn; one pass per adapter that the tile
+// holds and 64 rank rows.
+constexpr int kShrinkManyWaves = 4;
+struct ShrinkManyParams {
+  ShrinkParams s;
+  const uint32_t* order;
+};
+
+template <int XT, int AT>
+__global__ __launch_bounds__(kShrinkManyWaves* kWave) void shrink_many_kernel(ShrinkManyParams sp) {
+  const ShrinkParams& p = sp.s;
+  constexpr int NX = kTerms<XT>, NA = kTerms<AT>, JB = 4;
+  __shared__ float part[kShrinkManyWaves][JB][4][kWave];
+  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, K = p.words * 8u;
+  const uint32_t i0 = blockIdx.x * 16u, j0 = blockIdx.y * 64u;
+  const uint32_t i = i0 + lane % 16u, slot = lane / 16u;
+  const uint32_t t = i < p.tokens ? (sp.order ? sp.order[i] : i) : 0u;
+  uint32_t a = 0;
+  const uint32_t rank = i < p.tokens ? token_rank(p.ad, p.ids, t, a) : 0u;
+  const size_t xo = t * p.stride + 8u * slot;
+  uint64_t left = __ballot(rank != 0u) & 0xFFFFull;
+  while (left) {
+    const int leader = __builtin_ctzll(left);
+    const uint32_t aa = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a), leader));
+    const uint32_t rr = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), leader));
+    const uint64_t same = __ballot(rank != 0u && a == aa) & 0xFFFFull;
+    left &= ~same;
+    f32x4 acc[JB];
+#pragma unroll
+    for (int b = 0; b < JB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint32_t blocks = rr > j0 ? (rr - j0 + 15u) / 16u : 0u;  // of 16 rank rows; those past the rank repeat its last
+    for (uint32_t k = wave * 32u; k < K; k += kShrinkManyWaves * 32u) {
+      float v[8];
+      load8<XT>(p.x, xo + k, p.x_wide, v);
+      bf16x8 xt[NX];
+      split_terms(v, xt);
+#pragma unroll
+      for (int b = 0; b < JB; ++b) {
+        if (static_cast<uint32_t>(b) >= blocks) break;
+        const uint32_t j = j0 + 16u * b + lane % 16u;
+        const size_t ao = (static_cast<size_t>(aa) * p.ad.max_rank + (j < rr ? j : rr - 1u)) * K + 8u * slot + k;
+        load8<AT>(p.ad.a, ao, p.a_wide, v);
+        bf16x8 at[NA];
+        split_terms(v, at);
+        acc[b] = mfma_terms(xt, at, acc[b]);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < JB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave][b][e][lane] = acc[b][e];
+    __syncthreads();
+    const float scale = p.ad.scales ? p.ad.scales[aa] : 1.0f;
+    for (uint32_t o = threadIdx.x; o < 16u * 64u; o += kShrinkManyWaves * kWave) {
+      const uint32_t r = o / 64u, j = o % 64u;
+      if (!((same >> r) & 1u) || j0 + j >= p.vr) continue;
+      const uint32_t l = r / 4u * 16u + j % 16u;
+      float y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kShrinkManyWaves; ++w) y += part[w][j / 16u][r % 4u][l];
+      p.v[static_cast<size_t>(i0 + r) * p.vr + j0 + j] = j0 + j < rr ? y * scale : 0.0f;
+    }
+    __syncthreads();
+  }
+}
+
+struct ManyParams {
+  ProjectParams p;
+  ManyPrepared many;
+  const uint32_t* order;
+  uint32_t bias_terms, tiles;
+};
+
+// Row n's columns j .. j + 7 of adapter a's B as bf16 terms, zero from the
+// rank on.
+template <int NB>
+__device__ __forceinline__ void expand_operand(const ProjectParams& p, uint32_t a, uint32_t n, uint32_t j, uint32_t rank,
+                                               bf16x8 (&t)[NB]) {
+  const size_t o = (static_cast<size_t>(a) * p.w.out_dim + n) * p.ad.max_rank + j;
+  float v[8];
+  if (p.b_wide && j + 8u <= p.ad.max_rank) {
+    if (p.ad.dtype == OSM_META_BF16)
+      load8<OSM_META_BF16>(p.ad.b, o, true, v);
+    else if (p.ad.dtype == OSM_META_F16)
+      load8<OSM_META_F16>(p.ad.b, o, true, v);
+    else
+      load8<OSM_META_F32>(p.ad.b, o, true, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = j + k < rank ? v[k] : 0.0f;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = j + k < rank ? adapter_element(p.ad, o + k) : 0.0f;
+  }
+  split_terms(v, t);
+}
+
+// SK columns a stage, sub-groups of 8 * GW * 2 columns. WM x WN wavefronts of
+// MT token tiles and NB row blocks each.
+template <int NT, int MT, int NB, int WM, int WN, int GW, int SK>
+__global__ __launch_bounds__(WM* WN* kWave, (WM * WN >= 8 ? 2 : 1)) void project_many_kernel(ManyParams mp) {
+  const ProjectParams& p = mp.p;
+  constexpr uint32_t TH = WM * WN * kWave;
+  constexpr uint32_t SC = 16u * GW, SUBS = SK / SC, STEPS = SK / 16;
+  constexpr uint32_t kTiles = WM * MT, kRows = WN * NB * 32u, kCh = SK / 32;  // kCh: 16-byte chunks of a row
+  constexpr uint32_t kXUnits = kTiles * STEPS * NT * kWave, kWUnits = kRows * kCh;
+  constexpr uint32_t kXPer = kXUnits / TH, kWPer = (kWUnits + TH - 1u) / TH;
+  static_assert(kXUnits % TH == 0, "whole units");
+  __shared__ uint4 xl[2][kXUnits];
+  __shared__ uint4 wl[2][kWUnits];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, wm = wave % WM, wn = wave / WM;
+  const uint32_t row = lane % 32u, slot = lane / 32u;
+  const uint32_t N = p.w.out_dim, words = p.w.packed_cols, steps = words / 2u, subs = words * 8u / SC;
+  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of the row
+  // blocks, so that its L2 holds their words for all token tiles.
+  const uint32_t tgrid = (mp.tiles + kTiles - 1u) / kTiles, ngrid = (N + kRows - 1u) / kRows;
+  uint32_t b = blockIdx.x;
+  {
+    const uint32_t total = tgrid * ngrid, per = total / 8u, rest = total % 8u, x = b % 8u, y = b / 8u;
+    b = x * per + (x < rest ? x : rest) + y;
+  }
+  const uint32_t tile0 = b % tgrid * kTiles, n0 = b / tgrid * kRows;
+  const uint4* frag = reinterpret_cast<const uint4*>(p.in.frag);
+
+  uint4 xr[kXPer], wr[kWPer];
+  auto fetch = [&](uint32_t st) {
+#pragma unroll
+    for (uint32_t i = 0; i < kXPer; ++i) {
+      const uint32_t u = tid + i * TH, m = u / (STEPS * NT * kWave), o = u % (STEPS * NT * kWave);
+      const uint32_t tile = tile0 + m < mp.tiles ? tile0 + m : mp.tiles - 1u;
+      // A stage may reach past the last step: the last is read again, and not used.
+      const uint32_t at = st * STEPS * NT * kWave + o, end = steps * NT * kWave;
+      xr[i] = ldg16(frag + static_cast<size_t>(tile) * end + (at < end ? at : at % kWave + end - kWave));
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kWPer; ++i) {
+      const uint32_t u = tid + i * TH, r = u / kCh, c = u % kCh + st * kCh;
+      const uint32_t n = n0 + r < N ? n0 + r : N - 1u;
+      wr[i] = ldg16(p.w.packed + static_cast<size_t>(n) * words + 4u * (c < words / 4u ? c : words / 4u - 1u));
+    }
+  };
+  auto stash = [&](uint32_t buf) {
+#pragma unroll
+    for (uint32_t i = 0; i < kXPer; ++i) xl[buf][tid + i * TH] = xr[i];
+#pragma unroll
+    for (uint32_t i = 0; i < kWPer; ++i) {
+      const uint32_t u = tid + i * TH, r = u / kCh, c = u % kCh;
+      if (kWUnits % TH == 0 || u < kWUnits) wl[buf][r * kCh + (c ^ (r % kCh))] = wr[i];
+    }
+  };
+
+  uint32_t nrow[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const uint32_t n = n0 + (wn * NB + nb) * 32u + row;
+    nrow[nb] = n < N ? n : N - 1u;
+  }
+  fetch(0u);
+  f32x16 total[NB][MT];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) total[nb][m][i] = 0.0f;
+  // The biases' part.
+  for (uint32_t kg = 0; kg < mp.many.kgs; ++kg) {
+    bf16x8 xs[MT][kSumTerms];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < kSumTerms; ++t) {
+        const uint32_t tl = tile0 + wm * MT + m, tile = tl < mp.tiles ? tl : mp.tiles - 1u;
+        xs[m][t] = __builtin_bit_cast(
+            bf16x8, ldg<u32x4>(mp.many.sum_frag + (((static_cast<size_t>(tile) * mp.many.kgs + kg) * kSumTerms + t) * kWave + lane) * 8u));
+      }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t blk = n0 / 32u + wn * NB + nb, last = (N - 1u) / 32u;
+      const __bf16* bf = mp.many.bias_frag +
+                         (static_cast<size_t>(blk < last ? blk : last) * mp.many.kgs + kg) * mp.bias_terms * kWave * 8u + lane * 8u;
+      for (uint32_t j = 0; j < mp.bias_terms; ++j) {
+        const bf16x8 bt = __builtin_bit_cast(bf16x8, ldg<u32x4>(bf + j * kWave * 8u));
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int t = 0; t < kSumTerms; ++t)
+            if (t + j < 3u) total[nb][m] = mfma_bf16(xs[m][t], bt, total[nb][m]);
+      }
+    }
+  }
+  stash(0u);
   __syncthreads();
-  for (uint32_t o = threadIdx.x; o < MT * R * R; o += kFewWaves * kWave) {
-    const uint32_t t = o / R, nn = n0 + o % R, tr = t % R, m = t / R;
-    if (t >= p.tokens || nn >= N) continue;
-    const uint32_t i = R == 16 ? tr % 4u : tr / 8u * 4u + tr % 4u;
-    const uint32_t l = (R == 16 ? tr / 4u : tr / 4u % 2u) * R + o % R;
-    float y = 0.0f;
+  const uint32_t stages = (subs + SUBS - 1u) / SUBS;
+  for (uint32_t st = 0; st < stages; ++st) {
+    const uint32_t buf = st & 1u;
+    float sc[SUBS][NB];
 #pragma unroll
-    for (int k = 0; k < kFewWaves; ++k) y += part[k][m][i][l];
-    y = ldexpf(y, p.in.exps[t]);
-    if (p.ad.count) y += expand_one(p, t, nn);
-    store_out(p.y, p.y_dtype, t * p.y_stride + nn, y);
+    for (uint32_t u = 0; u < SUBS; ++u) {
+      const uint32_t sub = st * SUBS + u < subs ? st * SUBS + u : subs - 1u;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) sc[u][nb] = mp.many.scales[static_cast<size_t>(sub) * N + nrow[nb]];
+    }
+    if (st + 1u < stages) fetch(st + 1u);
+#pragma unroll
+    for (uint32_t u = 0; u < SUBS; ++u) {
+      if (SUBS > 1u && st * SUBS + u >= subs) break;
+      f16x8 q[NB][GW];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t r = (wn * NB + nb) * 32u + row, word = (u * 2u + slot) * GW;
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(&wl[buf][r * kCh + ((word / 4u) ^ (r % kCh))]) + word % 4u;
+        if constexpr (GW == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(at);
+          q[nb][0] = nibble_operand(v.x), q[nb][1] = nibble_operand(v.y), q[nb][2] = nibble_operand(v.z), q[nb][3] = nibble_operand(v.w);
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(at);
+          q[nb][0] = nibble_operand(v.x), q[nb][1] = nibble_operand(v.y);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        f32x16 d[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d[nb][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < GW; ++k)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const f16x8 a = __builtin_bit_cast(f16x8, xl[buf][(((wm * MT + m) * STEPS + u * GW + k) * NT + t) * kWave + lane]);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) d[nb] = Tile<32>::mfma(a, q[nb][k], d[nb]);
+          }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) total[nb][m][i] = fmaf(sc[u][nb], d[nb][i], total[nb][m][i]);
+      }
+    }
+    if (st + 1u < stages) stash(buf ^ 1u);  // last read a stage ago, before the barrier below
+    __syncthreads();
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const uint32_t tile = tile0 + wm * MT + m;
+    if (tile >= mp.tiles) break;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = p.in.exps[tile * 32u + Tile<32>::row(lane, i)];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) total[nb][m][i] = ldexpf(total[nb][m][i], e);
+    }
+    if (p.ad.count) {
+      // One product per adapter that the tile's tokens have, added to its own tokens' rows.
+      const uint32_t i = tile * 32u + row;
+      uint32_t a = 0, rank = 0;
+      if (i < p.tokens) rank = token_rank(p.ad, p.ids, mp.order ? mp.order[i] : i, a);
+      const float* v = p.in.v + static_cast<size_t>(i < p.tokens ? i : 0u) * p.in.vr + 8u * slot;
+      uint32_t left = static_cast<uint32_t>(__ballot(rank != 0u));
+      while (left) {
+        const int leader = __builtin_ctz(left);
+        const uint32_t aa = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a), leader));
+        const uint32_t rr = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), leader));
+        const uint32_t same = static_cast<uint32_t>(__ballot(rank != 0u && a == aa));
+        left &= ~same;
+        f32x16 e[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) e[nb][k] = 0.0f;
+        for (uint32_t j = 0; j < rr; j += 16u) {
+          float c[8];
+          load8<OSM_META_F32>(v, j, true, c);
+          bf16x8 vt[3];
+          split_terms(c, vt);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            if (p.ad.dtype == OSM_META_BF16) {
+              bf16x8 bt[1];
+              expand_operand(p, aa, nrow[nb], j + 8u * slot, rr, bt);
+              e[nb] = mfma_terms(vt, bt, e[nb]);
+            } else {
+              bf16x8 bt[3];
+              expand_operand(p, aa, nrow[nb], j + 8u * slot, rr, bt);
+              e[nb] = mfma_terms(vt, bt, e[nb]);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const bool own = (same >> Tile<32>::row(lane, k)) & 1u;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) total[nb][m][k] += own ? e[nb][k] : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t o = tile * 32u + Tile<32>::row(lane, i);
+      if (o >= p.tokens) continue;
+      const size_t t = mp.order ? mp.order[o] : o;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t n = n0 + (wn * NB + nb) * 32u + row;
+        if (n < N) store_out(p.y, p.y_dtype, t * p.y_stride + n, total[nb][m][i]);
+      }
+    }
   }
 }
 
@@ -449,35 +1043,207 @@ int by_dtype(uint32_t dtype, F f) {
   }
 }
 
+constexpr uint32_t kVecTokens = 4;
 constexpr uint32_t kFewTokens = 64;
 
 uint32_t round_up(uint32_t n, uint32_t m) { return (n + m - 1u) / m * m; }
 size_t align256(size_t n) { return (n + 255u) & ~static_cast<size_t>(255u); }
 
-// What a call runs: the columns of a sub-group (0: a group that is no
-// multiple of 32, one kernel for any) and the tile.
+// What a call runs. sub_cols: columns of a sub-group, 0 where a group is no
+// multiple of 32 (one kernel for any).
+enum class Path { kAny, kVec, kFew, kMany };
 struct Plan {
-  uint32_t sub_cols, tile, rows, terms, vr;
-  size_t frag, sums, exps, v, total;  // workspace offsets
+  Path path;
+  bool sort;
+  uint32_t sub_cols, tile, rows, terms, vr, kgs, bias_terms;
+  size_t frag, sums, exps, scales, biases, order, offsets, v, total;  // workspace offsets
 };
 Plan plan_of(const osmd_project_args& a) {
   Plan p{};
-  const uint32_t G = a.w.group, K = a.w.packed_cols * 8u;
+  const uint32_t G = a.w.group, K = a.w.packed_cols * 8u, N = a.w.out_dim;
   p.vr = a.adapters.count ? round_up(a.adapters.max_rank, 16u) : 0u;
-  if (G % 32u == 0u && a.tokens <= kFewTokens) {
-    p.sub_cols = G % 128u == 0u ? 128u : G % 64u == 0u ? 64u : 32u;
-    p.tile = a.tokens <= 16u ? 16u : 32u;
+  p.path = G % 32u != 0u             ? Path::kAny
+           : a.tokens <= kVecTokens ? Path::kVec
+           : a.tokens <= kFewTokens ? Path::kFew
+                                    : Path::kMany;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  if (p.path == Path::kFew || p.path == Path::kMany) {
+    // Tiles of 16 up to 16 tokens, and where tiles of 32 would give fewer
+    // workgroups than compute units (37 fp32 tokens through 2048 x 4096: 16
+    // us with 32, 11.5 with 16; 64 bf16 ones through 12289 x 2048: 23 and 30).
+    p.tile = p.path == Path::kMany || (a.tokens > 16u && (N + 31u) / 32u * ((a.tokens + 31u) / 32u) >= 256u) ? 32u : 16u;
+    // Tiles of 32 have no registers for the operands of 128 columns.
+    p.sub_cols = G % 128u == 0u && p.tile == 16u ? 128u : G % 64u == 0u ? 64u : 32u;
     p.rows = round_up(a.tokens, p.tile);
     p.terms = a.x_dtype == OSM_META_F32 ? 2u : 1u;
-    p.sums = align256(static_cast<size_t>(p.rows) * K * 2u * p.terms);
-    p.exps = p.sums + align256(static_cast<size_t>(p.rows) * (K / p.sub_cols) * 4u);
-    p.v = p.exps + align256(static_cast<size_t>(p.rows) * 4u);
+    p.frag = take(static_cast<size_t>(p.rows) * K * 2u * p.terms);
+    const uint32_t subs = K / p.sub_cols;
+    p.exps = take(static_cast<size_t>(p.rows) * 4u);
+    if (p.path == Path::kFew) {
+      p.sums = take(static_cast<size_t>(p.rows) * subs * 4u);
+    } else {
+      p.kgs = (subs + 15u) / 16u;
+      p.bias_terms = a.w.meta_dtype == OSM_META_BF16 ? 1u : a.w.meta_dtype == OSM_META_F16 ? 2u : 3u;
+      p.sums = take(static_cast<size_t>(p.rows) * p.kgs * 16u * kSumTerms * 2u);
+      p.scales = take(static_cast<size_t>(subs) * N * 4u);
+      p.biases = take(static_cast<size_t>(round_up(N, 32u)) * p.kgs * 16u * p.bias_terms * 2u);
+      p.sort = a.adapters.count > 1u && a.adapters.count <= OSMD_GROUP_MAX_BUCKETS;
+      if (p.sort) {
+        p.order = take(static_cast<size_t>(a.tokens) * 4u);
+        p.offsets = take((static_cast<size_t>(a.adapters.count) + 1u) * 4u);
+      }
+    }
   }
-  p.total = p.v + static_cast<size_t>(a.tokens) * p.vr * sizeof(float);
+  p.v = take(static_cast<size_t>(a.tokens) * p.vr * sizeof(float));
+  p.total = at;
   return p;
 }
 
-template <int R, int GW, int MT>
+Prepared prepared_of(const Plan& pl, uint8_t* work) {
+  Prepared out;
+  out.frag = reinterpret_cast<_Float16*>(work + pl.frag);
+  out.sums = reinterpret_cast<float*>(work + pl.sums);
+  out.exps = reinterpret_cast<int32_t*>(work + pl.exps);
+  out.v = reinterpret_cast<float*>(work + pl.v);
+  out.vr = pl.vr;
+  return out;
+}
+
+ShrinkParams shrink_params(const osmd_project_args& a, const Plan& pl, uint8_t* work) {
+  ShrinkParams sp{};
+  sp.x = a.x;
+  sp.stride = a.x_stride;
+  sp.tokens = a.tokens;
+  sp.words = a.w.packed_cols;
+  sp.x_wide = wide_rows(a.x, a.x_stride, a.x_dtype) ? 1u : 0u;
+  sp.a_wide = wide_rows(a.adapters.a, 8u * a.w.packed_cols, a.adapters.dtype) ? 1u : 0u;
+  sp.ad = a.adapters;
+  sp.ids = a.adapter_ids;
+  sp.v = prepared_of(pl, work).v;
+  sp.vr = pl.vr;
+  return sp;
+}
+
+ProjectParams project_params(const osmd_project_args& a, const Plan& pl, uint8_t* work) {
+  ProjectParams p{};
+  p.w = a.w;
+  p.groups = a.w.packed_cols * 8u / a.w.group;
+  p.per_group = pl.sub_cols ? a.w.group / pl.sub_cols : 1u;
+  p.in = prepared_of(pl, work);
+  p.y = a.y;
+  p.y_stride = a.y_stride;
+  p.y_dtype = a.y_dtype;
+  p.tokens = a.tokens;
+  p.ad = a.adapters;
+  p.ids = a.adapter_ids;
+  p.b_wide = wide_rows(a.adapters.b, a.adapters.max_rank, a.adapters.dtype) ? 1u : 0u;
+  return p;
+}
+
+int launch_shrink(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStream_t st) {
+  const ShrinkParams sp = shrink_params(a, pl, work);
+  return by_dtype(a.x_dtype, [&](auto xt) {
+    return by_dtype(a.adapters.dtype, [&](auto at) {
+      shrink_kernel<decltype(xt)::value, decltype(at)::value>
+          <<<a.tokens * (pl.vr / kShrinkWaves), kShrinkWaves * kWave, 0, st>>>(sp);
+      return launch_status();
+    });
+  });
+}
+
+template <int GW>
+int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStream_t st) {
+  ManyParams mp{};
+  mp.p = project_params(a, pl, work);
+  mp.tiles = pl.rows / 32u;
+  mp.bias_terms = pl.bias_terms;
+  mp.many.sum_frag = reinterpret_cast<__bf16*>(work + pl.sums);
+  mp.many.scales = reinterpret_cast<float*>(work + pl.scales);
+  mp.many.bias_frag = reinterpret_cast<__bf16*>(work + pl.biases);
+  mp.many.kgs = pl.kgs;
+  int r = 0;
+  if (pl.sort) {
+    // Tokens by adapter: a tile then holds one, or the few whose runs meet in it.
+    uint32_t* order = reinterpret_cast<uint32_t*>(work + pl.order);
+    r = osmd_group_rows(a.adapter_ids, a.tokens, a.adapters.count, reinterpret_cast<uint32_t*>(work + pl.offsets), order, st);
+    if (r != 0) return r;
+    mp.order = order;
+  }
+  PrepareManyParams pp{};
+  pp.x.x = a.x;
+  pp.x.stride = a.x_stride;
+  pp.x.tokens = a.tokens;
+  pp.x.rows = pl.rows;
+  pp.x.words = a.w.packed_cols;
+  pp.x.wide = wide_rows(a.x, a.x_stride, a.x_dtype) ? 1u : 0u;
+  pp.x.order = mp.order;
+  pp.x.out = mp.p.in;
+  pp.many = mp.many;
+  pp.w = a.w;
+  pp.groups = mp.p.groups;
+  pp.per_group = mp.p.per_group;
+  pp.subs = a.w.packed_cols * 8u / pl.sub_cols;
+  pp.x_blocks = pl.rows / 8u;
+  const uint32_t meta_blocks = (a.w.out_dim + 31u) / 32u * pl.kgs;
+  r = by_dtype(a.x_dtype, [&](auto xt) {
+    return by_dtype(a.w.meta_dtype, [&](auto meta) {
+      prepare_many_kernel<decltype(xt)::value, GW, decltype(meta)::value><<<pp.x_blocks + meta_blocks, 256, 0, st>>>(pp);
+      return launch_status();
+    });
+  });
+  if (r != 0) return r;
+  if (a.adapters.count) {
+    ShrinkManyParams sp{shrink_params(a, pl, work), mp.order};
+    r = by_dtype(a.x_dtype, [&](auto xt) {
+      return by_dtype(a.adapters.dtype, [&](auto at) {
+        shrink_many_kernel<decltype(xt)::value, decltype(at)::value>
+            <<<dim3((a.tokens + 15u) / 16u, (pl.vr + 63u) / 64u), kShrinkManyWaves * kWave, 0, st>>>(sp);
+        return launch_status();
+      });
+    });
+    if (r != 0) return r;
+  }
+  auto go = [&](auto kernel, uint32_t tiles, uint32_t rows, uint32_t threads) {
+    const uint32_t grid = (mp.tiles + tiles - 1u) / tiles * ((a.w.out_dim + rows - 1u) / rows);
+    kernel<<<grid, threads, 0, st>>>(mp);
+    return launch_status();
+  };
+  const bool big = (mp.tiles + 3u) / 4u * ((a.w.out_dim + 255u) / 256u) >= 256u;
+  if (pl.terms == 2u)
+    return big ? go(project_many_kernel<2, 2, 2, 2, 4, GW, 64>, 4u, 256u, 512u)
+               : go(project_many_kernel<2, 1, 1, 2, 4, GW, 128>, 2u, 128u, 512u);
+  return big ? go(project_many_kernel<1, 2, 2, 2, 4, GW, 128>, 4u, 256u, 512u)
+             : go(project_many_kernel<1, 1, 1, 2, 4, GW, 256>, 2u, 128u, 512u);
+}
+
+int launch_vec(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStream_t st) {
+  VecParams vp{};
+  vp.p = project_params(a, pl, work);
+  vp.x = a.x;
+  vp.stride = a.x_stride;
+  vp.wide = wide_rows(a.x, a.x_stride, a.x_dtype) ? 1u : 0u;
+  return by_dtype(a.w.meta_dtype, [&](auto meta) {
+    return by_dtype(a.x_dtype, [&](auto xt) {
+      constexpr int M = decltype(meta)::value, X = decltype(xt)::value;
+      auto go = [&](auto kernel, uint32_t rows, uint32_t tokens) {
+        const uint32_t per = kVecWaves * rows;
+        kernel<<<dim3((a.w.out_dim + per - 1u) / per, (a.tokens + tokens - 1u) / tokens), kVecWaves * kWave, 0, st>>>(vp);
+      };
+      if (a.tokens == 1u)
+        go(project_vec_kernel<M, X, 1, 4>, 4u, 1u);
+      else
+        go(project_vec_kernel<M, X, 2, 4>, 4u, 2u);
+      return launch_status();
+    });
+  });
+}
+
+template <int R, int GW>
 int launch_few(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStream_t st) {
   PrepareParams pp{};
   pp.x = a.x;
@@ -486,22 +1252,8 @@ int launch_few(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStr
   pp.rows = pl.rows;
   pp.words = a.w.packed_cols;
   pp.wide = wide_rows(a.x, a.x_stride, a.x_dtype) ? 1u : 0u;
-  pp.out.frag = reinterpret_cast<_Float16*>(work + pl.frag);
-  pp.out.sums = reinterpret_cast<float*>(work + pl.sums);
-  pp.out.exps = reinterpret_cast<int32_t*>(work + pl.exps);
-  pp.out.v = reinterpret_cast<float*>(work + pl.v);
-  pp.out.vr = pl.vr;
-  ShrinkParams sp{};
-  sp.x = a.x;
-  sp.stride = a.x_stride;
-  sp.tokens = a.tokens;
-  sp.words = a.w.packed_cols;
-  sp.x_wide = pp.wide;
-  sp.a_wide = wide_rows(a.adapters.a, 8u * a.w.packed_cols, a.adapters.dtype) ? 1u : 0u;
-  sp.ad = a.adapters;
-  sp.ids = a.adapter_ids;
-  sp.v = pp.out.v;
-  sp.vr = pl.vr;
+  pp.out = prepared_of(pl, work);
+  const ShrinkParams sp = shrink_params(a, pl, work);
   const uint32_t shrink_blocks = a.tokens * (pl.vr / 4u);
   int r = by_dtype(a.x_dtype, [&](auto xt) {
     return by_dtype(a.adapters.dtype, [&](auto at) {
@@ -511,25 +1263,19 @@ int launch_few(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStr
     });
   });
   if (r != 0) return r;
-  ProjectParams p{};
-  p.w = a.w;
-  p.groups = a.w.packed_cols * 8u / a.w.group;
-  p.per_group = a.w.group / pl.sub_cols;
-  p.in = pp.out;
-  p.y = a.y;
-  p.y_stride = a.y_stride;
-  p.y_dtype = a.y_dtype;
-  p.tokens = a.tokens;
-  p.ad = a.adapters;
-  p.ids = a.adapter_ids;
-  p.b_wide = wide_rows(a.adapters.b, a.adapters.max_rank, a.adapters.dtype) ? 1u : 0u;
-  const uint32_t grid = (a.w.out_dim + R - 1u) / R;
+  ProjectParams p = project_params(a, pl, work);
+  const uint32_t per_chunk = pl.sub_cols / 32u, subs = a.w.packed_cols * 8u / pl.sub_cols;
+  const uint32_t most = 2048u / R / per_chunk;  // sub-groups that a stage holds
+  const uint32_t stages = (subs + most - 1u) / most;
+  p.stage_subs = (subs + stages - 1u) / stages;
+  while ((1u << p.stage_log2) < p.stage_subs * per_chunk) ++p.stage_log2;
+  const dim3 grid((a.w.out_dim + R - 1u) / R, pl.rows / R);
   return by_dtype(a.w.meta_dtype, [&](auto meta) {
     constexpr int M = decltype(meta)::value;
     if (pl.terms == 2u)
-      project_few_kernel<R, 2, MT, GW, M><<<grid, kFewWaves * kWave, 0, st>>>(p);
+      project_few_kernel<R, 2, GW, M><<<grid, kFewWaves * kWave, 0, st>>>(p);
     else
-      project_few_kernel<R, 1, MT, GW, M><<<grid, kFewWaves * kWave, 0, st>>>(p);
+      project_few_kernel<R, 1, GW, M><<<grid, kFewWaves * kWave, 0, st>>>(p);
     return launch_status();
   });
 }
@@ -544,39 +1290,20 @@ int osmd_q4_project(const osmd_project_args* a, void* workspace, osmd_stream s) 
   const hipStream_t st = static_cast<hipStream_t>(s);
   const Plan pl = plan_of(*a);
   uint8_t* work = static_cast<uint8_t*>(workspace);
-  if (pl.sub_cols) {
-    auto few = [&](auto gw16) {  // words of a slot with tiles of 16; of 32: twice
-      constexpr int W = decltype(gw16)::value;
-      if (pl.tile == 16u) return launch_few<16, W, 1>(*a, pl, work, st);
-      if (pl.rows == 32u) return launch_few<32, 2 * W, 1>(*a, pl, work, st);
-      return launch_few<32, 2 * W, 2>(*a, pl, work, st);
-    };
-    return pl.sub_cols == 128u  ? few(std::integral_constant<int, 4>{})
-           : pl.sub_cols == 64u ? few(std::integral_constant<int, 2>{})
-                                : few(std::integral_constant<int, 1>{});
+  if (pl.path == Path::kMany)
+    return pl.sub_cols == 64u ? launch_many<4>(*a, pl, work, st) : launch_many<2>(*a, pl, work, st);
+  if (pl.path == Path::kFew) {
+    if (pl.tile == 32u) return pl.sub_cols == 64u ? launch_few<32, 4>(*a, pl, work, st) : launch_few<32, 2>(*a, pl, work, st);
+    return pl.sub_cols == 128u  ? launch_few<16, 4>(*a, pl, work, st)
+           : pl.sub_cols == 64u ? launch_few<16, 2>(*a, pl, work, st)
+                                : launch_few<16, 1>(*a, pl, work, st);
   }
-  float* v = reinterpret_cast<float*>(work + pl.v);
   if (a->adapters.count) {
-    ShrinkParams sp{};
-    sp.x = a->x;
-    sp.stride = a->x_stride;
-    sp.tokens = a->tokens;
-    sp.words = a->w.packed_cols;
-    sp.x_wide = wide_rows(a->x, a->x_stride, a->x_dtype) ? 1u : 0u;
-    sp.a_wide = wide_rows(a->adapters.a, 8u * a->w.packed_cols, a->adapters.dtype) ? 1u : 0u;
-    sp.ad = a->adapters;
-    sp.ids = a->adapter_ids;
-    sp.v = v;
-    sp.vr = pl.vr;
-    const int r = by_dtype(a->x_dtype, [&](auto xt) {
-      return by_dtype(a->adapters.dtype, [&](auto at) {
-        shrink_kernel<decltype(xt)::value, decltype(at)::value>
-            <<<a->tokens * (pl.vr / kShrinkWaves), kShrinkWaves * kWave, 0, st>>>(sp);
-        return launch_status();
-      });
-    });
+    const int r = launch_shrink(*a, pl, work, st);
     if (r != 0) return r;
   }
+  if (pl.path == Path::kVec) return launch_vec(*a, pl, work, st);
+  const float* v = reinterpret_cast<const float*>(work + pl.v);
   const uint32_t blocks = (a->w.out_dim + kAnyWaves - 1u) / kAnyWaves;
   const uint32_t tiles = (a->tokens + kAnyTokens - 1u) / kAnyTokens;
   return by_dtype(a->w.meta_dtype, [&](auto meta) {
