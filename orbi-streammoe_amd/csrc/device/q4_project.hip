@@ -95,6 +95,35 @@ __device__ __forceinline__ void load8(const void* x, size_t o, bool wide, float 
   }
 }
 
+// Eight elements as loaded.
+template <int T>
+struct Raw8 {
+  uint32_t u[T == OSM_META_F32 ? 8 : 4];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (T == OSM_META_F32)
+      return __uint_as_float(u[i]);
+    else
+      return meta_widen<T>((u[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+  }
+};
+template <int T>
+__device__ __forceinline__ void load_raw8(const void* x, size_t o, bool wide, Raw8<T>& r) {
+  if (wide) {
+    const uint4 a = ldg16(static_cast<const uint8_t*>(x) + o * (T == OSM_META_F32 ? 4u : 2u));
+    r.u[0] = a.x, r.u[1] = a.y, r.u[2] = a.z, r.u[3] = a.w;
+    if constexpr (T == OSM_META_F32) {
+      const uint4 b = ldg16(static_cast<const float*>(x) + o + 4u);
+      r.u[4] = b.x, r.u[5] = b.y, r.u[6] = b.z, r.u[7] = b.w;
+    }
+  } else if constexpr (T == OSM_META_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.u[i] = meta_bits<T>(x, o + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.u[i] = meta_bits<T>(x, o + 2 * i) | (meta_bits<T>(x, o + 2 * i + 1) << 16);
+  }
+}
+
 // Whether rows of `stride` elements from p on can be read 16 bytes at a time.
 bool wide_rows(const void* p, size_t stride, uint32_t dtype) {
   return reinterpret_cast<uintptr_t>(p) % 16u == 0u && stride * osm_meta_bytes(dtype) % 16u == 0u;
@@ -123,43 +152,51 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
   const bool live = row < p.tokens;
   const uint32_t t = !live ? 0u : p.order ? p.order[row] : row;
   const size_t xo = t * p.stride;
-  float top = 0.0f;
-  if (live)
-    for (uint32_t w = i; w < p.words; w += TPT) {
-      float v[8];
-      load8<XT>(p.x, xo + 8u * w, p.wide, v);
+  // Up to kKeep units of 8 columns a thread are read once and kept; of longer
+  // rows every batch is read again for the second pass.
+  constexpr uint32_t kKeep = 8;
+  Raw8<XT> keep[kKeep];
+  auto batch = [&](uint32_t w0) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+    for (uint32_t u = 0; u < kKeep; ++u) {
+      const uint32_t w = w0 + u * TPT;
+      load_raw8<XT>(p.x, xo + 8u * (w < p.words ? w : p.words - 1u), p.wide, keep[u]);
     }
+  };
+  float top = 0.0f;
+  for (uint32_t w0 = i; w0 < p.words; w0 += kKeep * TPT) {
+    batch(w0);
+#pragma unroll
+    for (uint32_t u = 0; u < kKeep; ++u)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(keep[u].get(k)));
+  }
   if constexpr (TPT == 256) {
     top = wave_max(top);
     if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   } else {
-    static_assert(TPT == 32, "half a wavefront");
+    static_assert(TPT <= kWave, "within a wavefront");
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
+    for (int m = 1; m < TPT; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
   }
   if (row >= p.rows) return;
   const int e = 141 - static_cast<int>(__float_as_uint(top) >> 23);
   if (i == 0) p.out.exps[row] = 24 - e;
   const uint32_t tile = row / R, steps = p.words / kSlots<R>, subs = p.words / GWS;
-  // Whole groups of GWS lanes stay in the loop together (words is a multiple of GWS).
-  for (uint32_t w = i; w < p.words; w += TPT) {
-    float v[8];
-    if (live) {
-      load8<XT>(p.x, xo + 8u * w, p.wide, v);
-    } else {
+  for (uint32_t w0 = i; w0 < p.words; w0 += kKeep * TPT) {
+    if (p.words > kKeep * TPT) batch(w0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    }
+    for (uint32_t u = 0; u < kKeep; ++u) {
+    const uint32_t w = w0 + u * TPT;
+    if (w >= p.words) break;  // whole groups of GWS lanes leave together (words is a multiple of GWS)
     float sum = 0.0f;
     f16x8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       constexpr int nibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-      const float s = ldexpf(v[nibble[k]], e);
+      const float s = live ? ldexpf(keep[u].get(nibble[k]), e) : 0.0f;
       sum += s;
       const float o = (nibble[k] & 1) ? s * 0.0625f : s;
       hi[k] = static_cast<_Float16>(o);
@@ -179,6 +216,7 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
       }
     } else {
       if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
+    }
     }
   }
 }
@@ -609,6 +647,20 @@ __device__ __forceinline__ C mfma_terms(const bf16x8 (&a)[NA], const bf16x8 (&b)
   return c;
 }
 
+// The same of eight elements as loaded.
+template <int T, int NT>
+__device__ __forceinline__ void raw_terms(const Raw8<T>& r, bf16x8 (&t)[NT]) {
+  if constexpr (T == OSM_META_BF16) {
+    const u32x4 v = {r.u[0], r.u[1], r.u[2], r.u[3]};
+    t[0] = __builtin_bit_cast(bf16x8, v);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = r.get(k);
+    split_terms(v, t);
+  }
+}
+
 constexpr int kSumTerms = 3;
 
 struct ManyPrepared {
@@ -659,30 +711,30 @@ struct PrepareManyParams {
   uint32_t groups, per_group, subs, x_blocks;
 };
 
-template <int XT, int GW, int META>
+template <int XT, int GW, int META, int TPT>
 __global__ __launch_bounds__(256) void prepare_many_kernel(PrepareManyParams p) {
   if (blockIdx.x < p.x_blocks)
-    prepare_rows<XT, 32, GW, 32, true>(p.x, blockIdx.x, &p.many);
+    prepare_rows<XT, 32, GW, TPT, true>(p.x, blockIdx.x, &p.many);
   else
     prepare_meta<META>(p.w, p.groups, p.per_group, p.subs, p.many, blockIdx.x - p.x_blocks);
 }
 
 // v of tiles of 16 tokens (in `order`): x and A_a split into bf16 terms, the
-// wavefronts taking the columns in turn; one pass per adapter that the tile
-// holds and 64 rank rows.
-constexpr int kShrinkManyWaves = 4;
+// wavefronts taking the columns in turn, kSteps steps of loads in flight; one
+// pass per adapter that the tile holds and 16 JB rank rows.
+constexpr int kShrinkManyWaves = 8;
 struct ShrinkManyParams {
   ShrinkParams s;
   const uint32_t* order;
 };
 
-template <int XT, int AT>
+template <int XT, int AT, int JB>
 __global__ __launch_bounds__(kShrinkManyWaves* kWave) void shrink_many_kernel(ShrinkManyParams sp) {
   const ShrinkParams& p = sp.s;
-  constexpr int NX = kTerms<XT>, NA = kTerms<AT>, JB = 4;
+  constexpr int NX = kTerms<XT>, NA = kTerms<AT>, kSteps = JB == 1 ? 4 : 2;
   __shared__ float part[kShrinkManyWaves][JB][4][kWave];
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, K = p.words * 8u;
-  const uint32_t i0 = blockIdx.x * 16u, j0 = blockIdx.y * 64u;
+  const uint32_t i0 = blockIdx.x * 16u, j0 = blockIdx.y * 16u * JB;
   const uint32_t i = i0 + lane % 16u, slot = lane / 16u;
   const uint32_t t = i < p.tokens ? (sp.order ? sp.order[i] : i) : 0u;
   uint32_t a = 0;
@@ -696,23 +748,34 @@ __global__ __launch_bounds__(kShrinkManyWaves* kWave) void shrink_many_kernel(Sh
     const uint64_t same = __ballot(rank != 0u && a == aa) & 0xFFFFull;
     left &= ~same;
     f32x4 acc[JB];
+    size_t ao[JB];
 #pragma unroll
-    for (int b = 0; b < JB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint32_t blocks = rr > j0 ? (rr - j0 + 15u) / 16u : 0u;  // of 16 rank rows; those past the rank repeat its last
-    for (uint32_t k = wave * 32u; k < K; k += kShrinkManyWaves * 32u) {
-      float v[8];
-      load8<XT>(p.x, xo + k, p.x_wide, v);
-      bf16x8 xt[NX];
-      split_terms(v, xt);
+    for (int b = 0; b < JB; ++b) {
+      acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const uint32_t j = j0 + 16u * b + lane % 16u;  // rows past the rank repeat its last
+      ao[b] = (static_cast<size_t>(aa) * p.ad.max_rank + (j < rr ? j : rr - 1u)) * K + 8u * slot;
+    }
+    Raw8<XT> x[kSteps];
+    Raw8<AT> c[kSteps][JB];
+    for (uint32_t k0 = wave * 32u; k0 < K; k0 += kSteps * kShrinkManyWaves * 32u) {
 #pragma unroll
-      for (int b = 0; b < JB; ++b) {
-        if (static_cast<uint32_t>(b) >= blocks) break;
-        const uint32_t j = j0 + 16u * b + lane % 16u;
-        const size_t ao = (static_cast<size_t>(aa) * p.ad.max_rank + (j < rr ? j : rr - 1u)) * K + 8u * slot + k;
-        load8<AT>(p.ad.a, ao, p.a_wide, v);
-        bf16x8 at[NA];
-        split_terms(v, at);
-        acc[b] = mfma_terms(xt, at, acc[b]);
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t at = k0 + s * kShrinkManyWaves * 32u, k = at < K ? at : k0;
+        load_raw8<XT>(p.x, xo + k, p.x_wide, x[s]);
+#pragma unroll
+        for (int b = 0; b < JB; ++b) load_raw8<AT>(p.ad.a, ao[b] + k, p.a_wide, c[s][b]);
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (k0 + s * kShrinkManyWaves * 32u >= K) break;
+        bf16x8 xt[NX];
+        raw_terms(x[s], xt);
+#pragma unroll
+        for (int b = 0; b < JB; ++b) {
+          bf16x8 at[NA];
+          raw_terms(c[s][b], at);
+          acc[b] = mfma_terms(xt, at, acc[b]);
+        }
       }
     }
 #pragma unroll
@@ -721,8 +784,8 @@ __global__ __launch_bounds__(kShrinkManyWaves* kWave) void shrink_many_kernel(Sh
       for (int e = 0; e < 4; ++e) part[wave][b][e][lane] = acc[b][e];
     __syncthreads();
     const float scale = p.ad.scales ? p.ad.scales[aa] : 1.0f;
-    for (uint32_t o = threadIdx.x; o < 16u * 64u; o += kShrinkManyWaves * kWave) {
-      const uint32_t r = o / 64u, j = o % 64u;
+    for (uint32_t o = threadIdx.x; o < 16u * 16u * JB; o += kShrinkManyWaves * kWave) {
+      const uint32_t r = o / (16u * JB), j = o % (16u * JB);
       if (!((same >> r) & 1u) || j0 + j >= p.vr) continue;
       const uint32_t l = r / 4u * 16u + j % 16u;
       float y = 0.0f;
@@ -1188,11 +1251,20 @@ int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipSt
   pp.groups = mp.p.groups;
   pp.per_group = mp.p.per_group;
   pp.subs = a.w.packed_cols * 8u / pl.sub_cols;
-  pp.x_blocks = pl.rows / 8u;
+  // 32 or 64 threads a row while they hold it in registers, else the workgroup.
+  const uint32_t per_row = a.w.packed_cols <= 256u ? 32u : a.w.packed_cols <= 512u ? 64u : 256u;
+  pp.x_blocks = pl.rows * per_row / 256u;
   const uint32_t meta_blocks = (a.w.out_dim + 31u) / 32u * pl.kgs;
   r = by_dtype(a.x_dtype, [&](auto xt) {
     return by_dtype(a.w.meta_dtype, [&](auto meta) {
-      prepare_many_kernel<decltype(xt)::value, GW, decltype(meta)::value><<<pp.x_blocks + meta_blocks, 256, 0, st>>>(pp);
+      constexpr int X = decltype(xt)::value, M = decltype(meta)::value;
+      auto go = [&](auto kernel) { kernel<<<pp.x_blocks + meta_blocks, 256, 0, st>>>(pp); };
+      if (per_row == 32u)
+        go(prepare_many_kernel<X, GW, M, 32>);
+      else if (per_row == 64u)
+        go(prepare_many_kernel<X, GW, M, 64>);
+      else
+        go(prepare_many_kernel<X, GW, M, 256>);
       return launch_status();
     });
   });
@@ -1201,8 +1273,16 @@ int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipSt
     ShrinkManyParams sp{shrink_params(a, pl, work), mp.order};
     r = by_dtype(a.x_dtype, [&](auto xt) {
       return by_dtype(a.adapters.dtype, [&](auto at) {
-        shrink_many_kernel<decltype(xt)::value, decltype(at)::value>
-            <<<dim3((a.tokens + 15u) / 16u, (pl.vr + 63u) / 64u), kShrinkManyWaves * kWave, 0, st>>>(sp);
+        constexpr int X = decltype(xt)::value, A = decltype(at)::value;
+        auto go = [&](auto kernel, uint32_t ranks) {
+          kernel<<<dim3((a.tokens + 15u) / 16u, (pl.vr + ranks - 1u) / ranks), kShrinkManyWaves * kWave, 0, st>>>(sp);
+        };
+        if (pl.vr <= 16u)
+          go(shrink_many_kernel<X, A, 1>, 16u);
+        else if (pl.vr <= 32u)
+          go(shrink_many_kernel<X, A, 2>, 32u);
+        else
+          go(shrink_many_kernel<X, A, 4>, 64u);
         return launch_status();
       });
     });
