@@ -10,18 +10,11 @@ namespace {
 
 using namespace osmk;
 
-__device__ __forceinline__ uint16_t bf16_rne(float f) {
-  uint32_t u = __float_as_uint(f);
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return static_cast<uint16_t>((u >> 16) | 0x40u);
-  u += 0x7FFFu + ((u >> 16) & 1u);
-  return static_cast<uint16_t>(u >> 16);
-}
-
 __device__ __forceinline__ void store_out(void* y, uint32_t dtype, size_t i, float v) {
   if (dtype == OSM_META_F32)
     static_cast<float*>(y)[i] = v;
   else if (dtype == OSM_META_BF16)
-    static_cast<uint16_t*>(y)[i] = bf16_rne(v);
+    static_cast<__bf16*>(y)[i] = static_cast<__bf16>(v);
   else
     static_cast<_Float16*>(y)[i] = static_cast<_Float16>(v);
 }
@@ -105,6 +98,12 @@ struct Raw8 {
     else
       return meta_widen<T>((u[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
   }
+  __device__ __forceinline__ void clear(int i) {
+    if constexpr (T == OSM_META_F32)
+      u[i] = 0u;
+    else
+      u[i >> 1] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+  }
 };
 template <int T>
 __device__ __forceinline__ void load_raw8(const void* x, size_t o, bool wide, Raw8<T>& r) {
@@ -138,17 +137,19 @@ struct PrepareParams {
   Prepared out;
 };
 
-// TPT threads per row, 256 / TPT rows per workgroup.
 struct ManyPrepared;
+
 template <int TERMS>
 __device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v);
+__device__ __forceinline__ uint32_t many_columns(const ManyPrepared& m);
 
-template <int XT, int R, int GW, int TPT, bool MANY = false>
+// TPT threads a row, of a workgroup's THREADS.
+template <int XT, int R, int GW, int TPT, int THREADS = 256, bool MANY = false>
 __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t block, const ManyPrepared* many = nullptr) {
   constexpr int NT = XT == OSM_META_F32 ? 2 : 1;
   constexpr uint32_t GWS = GW * kSlots<R>;  // words of a sub-group
-  __shared__ float red[256 / kWave];
-  const uint32_t i = threadIdx.x % TPT, row = block * (256u / TPT) + threadIdx.x / TPT;
+  __shared__ float red[THREADS / kWave];
+  const uint32_t i = threadIdx.x % TPT, row = block * (THREADS / TPT) + threadIdx.x / TPT;
   const bool live = row < p.tokens;
   const uint32_t t = !live ? 0u : p.order ? p.order[row] : row;
   const size_t xo = t * p.stride;
@@ -171,13 +172,14 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
 #pragma unroll
       for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(keep[u].get(k)));
   }
-  if constexpr (TPT == 256) {
+  if constexpr (TPT > kWave) {
+    static_assert(TPT == THREADS, "a row is a wavefront's part or the workgroup's");
     top = wave_max(top);
     if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int w = 0; w < THREADS / kWave; ++w) top = fmaxf(top, red[w]);
   } else {
-    static_assert(TPT <= kWave, "within a wavefront");
 #pragma unroll
     for (int m = 1; m < TPT; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
   }
@@ -212,7 +214,7 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
       if (iw == 0) {
         store_sum<3>(*many, tile, sub, row % R, sum * 0x1p-24f);
         if (sub + 1u == subs)
-          for (uint32_t z = subs; z % 16u != 0u; ++z) store_sum<3>(*many, tile, z, row % R, 0.0f);
+          for (uint32_t z = subs; z < many_columns(*many); ++z) store_sum<3>(*many, tile, z, row % R, 0.0f);
       }
     } else {
       if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
@@ -371,11 +373,16 @@ __device__ __forceinline__ float expand_one(const ProjectParams& p, uint32_t t, 
 
 constexpr int kFewWaves = 8;
 constexpr int kWaitVmcnt0 = 0x0F70;  // s_waitcnt operand: vector memory counter 0, the others at their maximum
+// Vector memory counter n and LDS counter 0.
+constexpr int wait_vm_lgkm(int n) { return (n & 15) | (n >> 4 << 14) | 7 << 4; }
 
 // 16 bytes per lane from global memory straight into LDS, lane l's at
 // dst + 16 l (dst wave-uniform).
 __device__ __forceinline__ void load_lds16(const void* src, void* dst) {
   __builtin_amdgcn_global_load_lds(src, dst, 16, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds(src, dst, 4, 0, 0);
 }
 
 // A stage is what a workgroup holds in LDS at a time: its R rows' words of
@@ -665,10 +672,15 @@ constexpr int kSumTerms = 3;
 
 struct ManyPrepared {
   __bf16* sum_frag;   // [tile][16 sub-groups][term][64][8]
-  float* scales;      // [sub-group][row of W]
+  float* scales;      // [sub-group][row of W, scale_row apart], then a row of zeros
+  uint32_t scale_row;
   __bf16* bias_frag;  // [32 rows][16 sub-groups][term][64][8]
   uint32_t kgs;       // runs of 16 sub-groups
+  __bf16* v_frag;     // [tile][16 rank rows][term][64][8]: v, scale_a A_a x
 };
+
+__device__ __forceinline__ uint32_t many_columns(const ManyPrepared& m) { return m.kgs * 16u; }
+__device__ __forceinline__ bf16x8 load_bf16(const __bf16* p) { return __builtin_bit_cast(bf16x8, ldg<u32x4>(p)); }
 
 template <int TERMS>
 __device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v) {
@@ -688,11 +700,12 @@ __device__ __forceinline__ void prepare_meta(const osmd_q4_proj& w, uint32_t gro
                                              const ManyPrepared& out, uint32_t block) {
   constexpr int NT = kTerms<META>;
   const uint32_t nb = block / out.kgs, kg = block % out.kgs;
-  for (uint32_t i = threadIdx.x; i < 512u; i += 256u) {
+  for (uint32_t i = threadIdx.x; i < 512u; i += blockDim.x) {
     const uint32_t r = i % 32u, s = i / 32u, n = nb * 32u + r, sub = kg * 16u + s;
     const bool in = n < w.out_dim && sub < subs;
     const size_t o = static_cast<size_t>(in ? n : 0u) * groups + (in ? sub / per_group : 0u);
-    if (in) out.scales[static_cast<size_t>(sub) * w.out_dim + n] = meta_at<META>(w.scales, o);
+    if (sub < subs) out.scales[static_cast<size_t>(sub) * out.scale_row + n] = in ? meta_at<META>(w.scales, o) : 0.0f;
+    if (sub == 0u) out.scales[static_cast<size_t>(subs) * out.scale_row + n] = 0.0f;
     float left = in ? meta_at<META>(w.biases, o) : 0.0f;
     const uint32_t lane = s / 8u * 32u + r;
 #pragma unroll
@@ -704,21 +717,6 @@ __device__ __forceinline__ void prepare_meta(const osmd_q4_proj& w, uint32_t gro
   }
 }
 
-struct PrepareManyParams {
-  PrepareParams x;
-  ManyPrepared many;
-  osmd_q4_proj w;
-  uint32_t groups, per_group, subs, x_blocks;
-};
-
-template <int XT, int GW, int META, int TPT>
-__global__ __launch_bounds__(256) void prepare_many_kernel(PrepareManyParams p) {
-  if (blockIdx.x < p.x_blocks)
-    prepare_rows<XT, 32, GW, TPT, true>(p.x, blockIdx.x, &p.many);
-  else
-    prepare_meta<META>(p.w, p.groups, p.per_group, p.subs, p.many, blockIdx.x - p.x_blocks);
-}
-
 // v of tiles of 16 tokens (in `order`): x and A_a split into bf16 terms, the
 // wavefronts taking the columns in turn, kSteps steps of loads in flight; one
 // pass per adapter that the tile holds and 16 JB rank rows.
@@ -726,15 +724,18 @@ constexpr int kShrinkManyWaves = 8;
 struct ShrinkManyParams {
   ShrinkParams s;
   const uint32_t* order;
+  __bf16* v_frag;
 };
 
 template <int XT, int AT, int JB>
-__global__ __launch_bounds__(kShrinkManyWaves* kWave) void shrink_many_kernel(ShrinkManyParams sp) {
+__device__ __forceinline__ void shrink_tile(const ShrinkManyParams& sp, uint32_t block) {
   const ShrinkParams& p = sp.s;
-  constexpr int NX = kTerms<XT>, NA = kTerms<AT>, kSteps = JB == 1 ? 4 : 2;
+  constexpr int NX = kTerms<XT>, NA = kTerms<AT>;
+  // Steps in flight: within some 100 registers.
+  constexpr int kSteps = JB == 1 ? 6 : AT == OSM_META_F32 ? 2 : 4;
   __shared__ float part[kShrinkManyWaves][JB][4][kWave];
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, K = p.words * 8u;
-  const uint32_t i0 = blockIdx.x * 16u, j0 = blockIdx.y * 16u * JB;
+  const uint32_t tiles = (p.tokens + 15u) / 16u, i0 = block % tiles * 16u, j0 = block / tiles * 16u * JB;
   const uint32_t i = i0 + lane % 16u, slot = lane / 16u;
   const uint32_t t = i < p.tokens ? (sp.order ? sp.order[i] : i) : 0u;
   uint32_t a = 0;
@@ -791,103 +792,201 @@ __global__ __launch_bounds__(kShrinkManyWaves* kWave) void shrink_many_kernel(Sh
       float y = 0.0f;
 #pragma unroll
       for (int w = 0; w < kShrinkManyWaves; ++w) y += part[w][j / 16u][r % 4u][l];
-      p.v[static_cast<size_t>(i0 + r) * p.vr + j0 + j] = j0 + j < rr ? y * scale : 0.0f;
+      // As the three bf16 terms that the tiled product reads.
+      y = j0 + j < rr ? y * scale : 0.0f;
+      const uint32_t it = i0 + r, jt = j0 + j, fl = jt % 16u / 8u * 32u + it % 32u;
+      __bf16* f = sp.v_frag + ((static_cast<size_t>(it / 32u) * (p.vr / 16u) + jt / 16u) * 3u * kWave + fl) * 8u + jt % 8u;
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        const __bf16 b = static_cast<__bf16>(y);
+        f[t * kWave * 8u] = b;
+        y -= static_cast<float>(b);
+      }
     }
     __syncthreads();
   }
+}
+
+// One launch before the tiled product: workgroups that shrink, then those that
+// prepare x, then W's scales and biases.
+struct PrepareManyParams {
+  ShrinkManyParams s;
+  PrepareParams x;
+  ManyPrepared many;
+  osmd_q4_proj w;
+  uint32_t groups, per_group, subs, shrink_blocks, x_blocks;
+};
+constexpr int kPrepareThreads = kShrinkManyWaves * kWave;
+
+template <int XT, int GW, int TPT, int AT, int JB>
+__global__ __launch_bounds__(kPrepareThreads) void prepare_many_kernel(PrepareManyParams p) {
+  if (blockIdx.x < p.shrink_blocks) return shrink_tile<XT, AT, JB>(p.s, blockIdx.x);
+  const uint32_t block = blockIdx.x - p.shrink_blocks;
+  if (block < p.x_blocks) return prepare_rows<XT, 32, GW, TPT, kPrepareThreads, true>(p.x, block, &p.many);
+  if (p.w.meta_dtype == OSM_META_F32)
+    prepare_meta<OSM_META_F32>(p.w, p.groups, p.per_group, p.subs, p.many, block - p.x_blocks);
+  else if (p.w.meta_dtype == OSM_META_F16)
+    prepare_meta<OSM_META_F16>(p.w, p.groups, p.per_group, p.subs, p.many, block - p.x_blocks);
+  else
+    prepare_meta<OSM_META_BF16>(p.w, p.groups, p.per_group, p.subs, p.many, block - p.x_blocks);
 }
 
 struct ManyParams {
   ProjectParams p;
   ManyPrepared many;
   const uint32_t* order;
-  uint32_t bias_terms, tiles;
+  uint32_t tiles;
+  uint32_t y_wide;  // 16-bit rows of y that 16 bytes at a time can be stored to
 };
 
-// Row n's columns j .. j + 7 of adapter a's B as bf16 terms, zero from the
-// rank on.
-template <int NB>
-__device__ __forceinline__ void expand_operand(const ProjectParams& p, uint32_t a, uint32_t n, uint32_t j, uint32_t rank,
-                                               bf16x8 (&t)[NB]) {
-  const size_t o = (static_cast<size_t>(a) * p.w.out_dim + n) * p.ad.max_rank + j;
-  float v[8];
-  if (p.b_wide && j + 8u <= p.ad.max_rank) {
-    if (p.ad.dtype == OSM_META_BF16)
-      load8<OSM_META_BF16>(p.ad.b, o, true, v);
-    else if (p.ad.dtype == OSM_META_F16)
-      load8<OSM_META_F16>(p.ad.b, o, true, v);
-    else
-      load8<OSM_META_F32>(p.ad.b, o, true, v);
+// e += v of the tile's tokens times B_a of the rows nrow, over the a's rank;
+// the next step's loads are on their way while one computes.
+template <int AT, int NB>
+__device__ __forceinline__ void expand_tile(const ProjectParams& p, uint32_t a, uint32_t rank, const __bf16* v_frag,
+                                            const uint32_t (&nrow)[NB], uint32_t slot, f32x16 (&e)[NB]) {
+  struct Step {
+    bf16x8 v[3];
+    Raw8<AT> b[NB];
+  } step[2];
+  const uint32_t R = p.ad.max_rank;
+  auto load = [&](Step& s, uint32_t j) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = j + k < rank ? v[k] : 0.0f;
-  } else {
+    for (int t = 0; t < 3; ++t) s.v[t] = load_bf16(v_frag + (j / 16u * 3u + t) * kWave * 8u);
+    const uint32_t c = j + 8u * slot;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = j + k < rank ? adapter_element(p.ad, o + k) : 0.0f;
+    for (int nb = 0; nb < NB; ++nb) {
+      const size_t o = (static_cast<size_t>(a) * p.w.out_dim + nrow[nb]) * R;
+      if (p.b_wide && R % 8u == 0u) {
+        load_raw8<AT>(p.ad.b, o + (c < R ? c : 0u), true, s.b[nb]);
+      } else {
+        // Rows that hold no whole pieces: element by element, the last one again past the end.
+        auto at = [&](uint32_t k) { return meta_bits<AT>(p.ad.b, o + (c + k < R ? c + k : R - 1u)); };
+        if constexpr (AT == OSM_META_F32) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) s.b[nb].u[k] = at(k);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s.b[nb].u[k] = at(2 * k) | (at(2 * k + 1) << 16);
+        }
+      }
+    }
+  };
+  auto compute = [&](const Step& s, uint32_t j) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      Raw8<AT> raw = s.b[nb];
+      if (j + 16u > rank) {  // zero from the rank on
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (j + 8u * slot + k >= rank) raw.clear(k);
+      }
+      bf16x8 bt[kTerms<AT>];
+      raw_terms(raw, bt);
+      e[nb] = mfma_terms(s.v, bt, e[nb]);
+    }
+  };
+  load(step[0], 0u);
+  for (uint32_t j = 0; j < rank; j += 32u) {
+    if (j + 16u < rank) load(step[1], j + 16u);
+    compute(step[0], j);
+    if (j + 16u >= rank) break;
+    if (j + 32u < rank) load(step[0], j + 32u);
+    compute(step[1], j + 16u);
   }
-  split_terms(v, t);
 }
 
-// SK columns a stage, sub-groups of 8 * GW * 2 columns. WM x WN wavefronts of
-// MT token tiles and NB row blocks each.
-template <int NT, int MT, int NB, int WM, int WN, int GW, int SK>
-__global__ __launch_bounds__(WM* WN* kWave, (WM * WN >= 8 ? 2 : 1)) void project_many_kernel(ManyParams mp) {
+// SK columns a stage, sub-groups of 16 * GW columns. WM x WN wavefronts of MT
+// token tiles and NB row blocks each, WK of them to a tile: they take a
+// stage's sub-groups in turn. RING stages in LDS: one computes while the next
+// are on their way into it, straight from memory. Each stage has an array of
+// its own: the compiler then knows that a stage's reads need not wait for the
+// loads into the others. The loop has no branch: it runs whole rounds of the
+// ring, stages past the last with scales of 0 on data read again.
+template <int META, int NT, int MT, int NB, int WM, int WN, int WK, int GW, int SK, int RING>
+__global__ __launch_bounds__(WM* WN* WK* kWave, 2) void project_many_kernel(ManyParams mp) {
   const ProjectParams& p = mp.p;
-  constexpr uint32_t TH = WM * WN * kWave;
-  constexpr uint32_t SC = 16u * GW, SUBS = SK / SC, STEPS = SK / 16;
+  constexpr int kBiasTerms = kTerms<META>;
+  constexpr uint32_t TH = WM * WN * WK * kWave;
+  constexpr uint32_t SC = 16u * GW, STEPS = SK / 16, SUBS = SK / SC / WK;  // SUBS: a wavefront's, of a stage
+  static_assert(SK % (SC * WK) == 0, "every wavefront takes as many sub-groups");
   constexpr uint32_t kTiles = WM * MT, kRows = WN * NB * 32u, kCh = SK / 32;  // kCh: 16-byte chunks of a row
   constexpr uint32_t kXUnits = kTiles * STEPS * NT * kWave, kWUnits = kRows * kCh;
-  constexpr uint32_t kXPer = kXUnits / TH, kWPer = (kWUnits + TH - 1u) / TH;
-  static_assert(kXUnits % TH == 0, "whole units");
-  __shared__ uint4 xl[2][kXUnits];
-  __shared__ uint4 wl[2][kWUnits];
-  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, wm = wave % WM, wn = wave / WM;
+  static_assert(kXUnits % TH == 0 && kWUnits % kWave == 0, "whole wavefronts");
+  static_assert(kWUnits % TH == 0 || TH % kWUnits == 0, "a round of words is every wavefront's, or repeated");
+  // Scales: a wavefront's own, 4 bytes a lane, two blocks of 32 rows a load.
+  static_assert(SUBS * NB % 2 == 0, "whole wavefronts");
+  constexpr uint32_t kWPer = (kWUnits + TH - 1u) / TH, kSPer = SUBS * NB / 2u;
+  constexpr int kLoads = kXUnits / TH + kWPer + kSPer;  // of a wavefront, a stage
+  constexpr uint32_t kStage = kXUnits + kWPer * TH + TH / kWave * kSPer * 16u;
+  __shared__ uint4 l0[kStage], l1[kStage], l2[kStage], l3[RING == 4 ? kStage : 1];
+  __shared__ uint32_t info[4][kTiles * 32u];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave;
+  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid / kWave)));
+  const uint32_t wm = wave % WM, wn = wave / WM % WN, wk = wave / (WM * WN);
   const uint32_t row = lane % 32u, slot = lane / 32u;
   const uint32_t N = p.w.out_dim, words = p.w.packed_cols, steps = words / 2u, subs = words * 8u / SC;
-  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of the row
-  // blocks, so that its L2 holds their words for all token tiles.
+  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of the tiles, so
+  // that its L2 holds what its compute units read. Of a run, 8 token tiles go
+  // through the row blocks together.
   const uint32_t tgrid = (mp.tiles + kTiles - 1u) / kTiles, ngrid = (N + kRows - 1u) / kRows;
   uint32_t b = blockIdx.x;
   {
     const uint32_t total = tgrid * ngrid, per = total / 8u, rest = total % 8u, x = b % 8u, y = b / 8u;
     b = x * per + (x < rest ? x : rest) + y;
   }
-  const uint32_t tile0 = b % tgrid * kTiles, n0 = b / tgrid * kRows;
+  const uint32_t band = b / (8u * ngrid), width = tgrid - band * 8u < 8u ? tgrid - band * 8u : 8u, in_band = b - band * 8u * ngrid;
+  const uint32_t tile0 = (band * 8u + in_band % width) * kTiles, n0 = in_band / width * kRows;
   const uint4* frag = reinterpret_cast<const uint4*>(p.in.frag);
-
-  uint4 xr[kXPer], wr[kWPer];
-  auto fetch = [&](uint32_t st) {
+  const uint32_t stages = (subs + SUBS * WK - 1u) / (SUBS * WK);
+  // The lane's chunks of words: row pointers and place in a stage's chunks.
+  const uint4* wrow[kWPer];
+  uint32_t wchunk[kWPer];
 #pragma unroll
-    for (uint32_t i = 0; i < kXPer; ++i) {
-      const uint32_t u = tid + i * TH, m = u / (STEPS * NT * kWave), o = u % (STEPS * NT * kWave);
-      const uint32_t tile = tile0 + m < mp.tiles ? tile0 + m : mp.tiles - 1u;
-      // A stage may reach past the last step: the last is read again, and not used.
-      const uint32_t at = st * STEPS * NT * kWave + o, end = steps * NT * kWave;
-      xr[i] = ldg16(frag + static_cast<size_t>(tile) * end + (at < end ? at : at % kWave + end - kWave));
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < kWPer; ++i) {
-      const uint32_t u = tid + i * TH, r = u / kCh, c = u % kCh + st * kCh;
-      const uint32_t n = n0 + r < N ? n0 + r : N - 1u;
-      wr[i] = ldg16(p.w.packed + static_cast<size_t>(n) * words + 4u * (c < words / 4u ? c : words / 4u - 1u));
-    }
-  };
-  auto stash = [&](uint32_t buf) {
-#pragma unroll
-    for (uint32_t i = 0; i < kXPer; ++i) xl[buf][tid + i * TH] = xr[i];
-#pragma unroll
-    for (uint32_t i = 0; i < kWPer; ++i) {
-      const uint32_t u = tid + i * TH, r = u / kCh, c = u % kCh;
-      if (kWUnits % TH == 0 || u < kWUnits) wl[buf][r * kCh + (c ^ (r % kCh))] = wr[i];
-    }
-  };
-
-  uint32_t nrow[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const uint32_t n = n0 + (wn * NB + nb) * 32u + row;
-    nrow[nb] = n < N ? n : N - 1u;
+  for (uint32_t i = 0; i < kWPer; ++i) {
+    // Chunk c of row r sits at r kCh + (c ^ (r % kCh)), which spreads the rows' equal chunks over the banks.
+    const uint32_t u = (tid + i * TH) % kWUnits, r = u / kCh;
+    const uint32_t n = n0 + r < N ? n0 + r : N - 1u;
+    wrow[i] = reinterpret_cast<const uint4*>(p.w.packed + static_cast<size_t>(n) * words);
+    wchunk[i] = (u % kCh) ^ (r % kCh);
   }
-  fetch(0u);
+  auto issue = [&](uint4* to, uint32_t st) {
+    // Scales (their rows are padded to whole workgroups').
+#pragma unroll
+    for (uint32_t i = 0; i < kSPer; ++i) {
+      // Block pair i: of NB = 2 sub-group i, of NB = 1 sub-groups 2 i and 2 i + 1.
+      const uint32_t u = NB == 2 ? i : 2u * i + slot, sub = (st * SUBS + u) * WK + wk;
+      const float* from = mp.many.scales + static_cast<size_t>(sub < subs ? sub : subs) * mp.many.scale_row + n0 +
+                          (NB == 2 ? wn * 64u + lane : wn * 32u + row);
+      load_lds4(from, to + (kXUnits + kWPer * TH + (wave * kSPer + i) * 16u));
+    }
+    // Fragments, 1 KB each; past a row's last step its last is read again.
+#pragma unroll
+    for (uint32_t i = 0; i < kXUnits / TH; ++i) {
+      const uint32_t f = i * (TH / kWave) + wave, m = f / (STEPS * NT), o = f % (STEPS * NT);
+      const uint32_t tile = tile0 + m < mp.tiles ? tile0 + m : mp.tiles - 1u;
+      const uint32_t at = st * STEPS * NT + o < steps * NT ? st * STEPS * NT + o : steps * NT - 1u;
+      load_lds16(frag + (static_cast<size_t>(tile) * steps * NT + at) * kWave + lane, to + f * kWave);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kWPer; ++i) {
+      const uint32_t c = wchunk[i] + st * kCh, last = words / 4u - 1u;
+      load_lds16(wrow[i] + (c < last ? c : last), to + (kXUnits + i * TH + wave * kWave));
+    }
+  };
+  issue(l0, 0u);
+  issue(l1, 1u);
+  issue(l2, 2u);
+  if constexpr (RING == 4) issue(l3, 3u);
+  // What the end needs of the tiles' tokens: place in y, exponent, adapter, rank.
+  for (uint32_t i = tid; i < kTiles * 32u; i += TH) {
+    const uint32_t at = tile0 * 32u + i;
+    uint32_t a = 0;
+    const uint32_t token = at < p.tokens ? (mp.order ? mp.order[at] : at) : 0u;
+    info[0][i] = token;
+    info[1][i] = at < p.tokens ? static_cast<uint32_t>(p.in.exps[at]) : 0u;
+    info[3][i] = p.ad.count && at < p.tokens ? token_rank(p.ad, p.ids, token, a) : 0u;
+    info[2][i] = a;
+  }
   f32x16 total[NB][MT];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -895,150 +994,268 @@ __global__ __launch_bounds__(WM* WN* kWave, (WM * WN >= 8 ? 2 : 1)) void project
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < 16; ++i) total[nb][m][i] = 0.0f;
-  // The biases' part.
-  for (uint32_t kg = 0; kg < mp.many.kgs; ++kg) {
-    bf16x8 xs[MT][kSumTerms];
+  // The biases' part, a run of sub-groups' operands on their way while one's
+  // products run.
+  {
+    struct Run {
+      bf16x8 x[MT][kSumTerms], b[NB][kBiasTerms];
+    } run[2];
+    const __bf16* xf[MT];
+    const __bf16* bf[NB];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+      const uint32_t tl = tile0 + wm * MT + m, tile = tl < mp.tiles ? tl : mp.tiles - 1u;
+      xf[m] = mp.many.sum_frag + (static_cast<size_t>(tile) * mp.many.kgs * kSumTerms * kWave + lane) * 8u;
+    }
 #pragma unroll
-      for (int t = 0; t < kSumTerms; ++t) {
-        const uint32_t tl = tile0 + wm * MT + m, tile = tl < mp.tiles ? tl : mp.tiles - 1u;
-        xs[m][t] = __builtin_bit_cast(
-            bf16x8, ldg<u32x4>(mp.many.sum_frag + (((static_cast<size_t>(tile) * mp.many.kgs + kg) * kSumTerms + t) * kWave + lane) * 8u));
-      }
+    for (int nb = 0; nb < NB; ++nb)
+      bf[nb] = mp.many.bias_frag + (static_cast<size_t>(n0 / 32u + wn * NB + nb) * mp.many.kgs * kBiasTerms * kWave + lane) * 8u;
+    auto load = [&](Run& r, uint32_t kg) {
+      const size_t at = kg < mp.many.kgs ? kg : mp.many.kgs - 1u;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t blk = n0 / 32u + wn * NB + nb, last = (N - 1u) / 32u;
-      const __bf16* bf = mp.many.bias_frag +
-                         (static_cast<size_t>(blk < last ? blk : last) * mp.many.kgs + kg) * mp.bias_terms * kWave * 8u + lane * 8u;
-      for (uint32_t j = 0; j < mp.bias_terms; ++j) {
-        const bf16x8 bt = __builtin_bit_cast(bf16x8, ldg<u32x4>(bf + j * kWave * 8u));
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int t = 0; t < kSumTerms; ++t) r.x[m][t] = load_bf16(xf[m] + (at * kSumTerms + t) * kWave * 8u);
 #pragma unroll
-          for (int t = 0; t < kSumTerms; ++t)
-            if (t + j < 3u) total[nb][m] = mfma_bf16(xs[m][t], bt, total[nb][m]);
-      }
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int t = 0; t < kBiasTerms; ++t) r.b[nb][t] = load_bf16(bf[nb] + (at * kBiasTerms + t) * kWave * 8u);
+    };
+    auto add = [&](const Run& r) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) total[nb][m] = mfma_terms(r.x[m], r.b[nb], total[nb][m]);
+    };
+    load(run[0], wk);
+    for (uint32_t kg = wk; kg < mp.many.kgs; kg += 2u * WK) {
+      load(run[1], kg + WK);
+      add(run[0]);
+      load(run[0], kg + 2u * WK);
+      if (kg + WK < mp.many.kgs) add(run[1]);
     }
   }
-  stash(0u);
-  __syncthreads();
-  const uint32_t stages = (subs + SUBS - 1u) / SUBS;
-  for (uint32_t st = 0; st < stages; ++st) {
-    const uint32_t buf = st & 1u;
-    float sc[SUBS][NB];
+  // Units of one sub-group and token tile: while one's matrix instructions
+  // run, the next one's operands come from LDS and the block before is scaled
+  // and added.
+  constexpr uint32_t kUnits = SUBS * MT;
+  static_assert(kUnits * NB % 2u == 0u, "blocks alternate between two sets of registers");
+  f16x8 x[2][GW * NT], q[NB][GW];
+  uint4 w[NB];
+  float scale[NB];
+  f32x16 d[2];
+  float before = 0.0f;  // the scale of the block before
 #pragma unroll
-    for (uint32_t u = 0; u < SUBS; ++u) {
-      const uint32_t sub = st * SUBS + u < subs ? st * SUBS + u : subs - 1u;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) sc[u][nb] = mp.many.scales[static_cast<size_t>(sub) * N + nrow[nb]];
-    }
-    if (st + 1u < stages) fetch(st + 1u);
-#pragma unroll
-    for (uint32_t u = 0; u < SUBS; ++u) {
-      if (SUBS > 1u && st * SUBS + u >= subs) break;
-      f16x8 q[NB][GW];
+  for (int i = 0; i < 16; ++i) d[1][i] = 0.0f;
+  auto load_unit = [&](const uint4* at, uint32_t j, f16x8 (&xx)[GW * NT]) {
+    const uint32_t u = j / MT, m = j % MT;
+    if (m == 0u) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t r = (wn * NB + nb) * 32u + row, word = (u * 2u + slot) * GW;
-        const uint32_t* at = reinterpret_cast<const uint32_t*>(&wl[buf][r * kCh + ((word / 4u) ^ (r % kCh))]) + word % 4u;
+        const uint32_t r = (wn * NB + nb) * 32u + row, word = ((u * WK + wk) * 2u + slot) * GW;
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(at + kXUnits + r * kCh + ((word / 4u) ^ (r % kCh))) + word % 4u;
         if constexpr (GW == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(at);
-          q[nb][0] = nibble_operand(v.x), q[nb][1] = nibble_operand(v.y), q[nb][2] = nibble_operand(v.z), q[nb][3] = nibble_operand(v.w);
+          w[nb] = *reinterpret_cast<const uint4*>(from);
         } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(at);
-          q[nb][0] = nibble_operand(v.x), q[nb][1] = nibble_operand(v.y);
+          const uint2 v = *reinterpret_cast<const uint2*>(from);
+          w[nb].x = v.x, w[nb].y = v.y;
         }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        f32x16 d[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) d[nb][i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < GW; ++k)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const f16x8 a = __builtin_bit_cast(f16x8, xl[buf][(((wm * MT + m) * STEPS + u * GW + k) * NT + t) * kWave + lane]);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) d[nb] = Tile<32>::mfma(a, q[nb][k], d[nb]);
-          }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) total[nb][m][i] = fmaf(sc[u][nb], d[nb][i], total[nb][m][i]);
+        scale[nb] = reinterpret_cast<const float*>(at + kXUnits + kWPer * TH + wave * kSPer * 16u)[(u * NB + nb) * 32u + row];
       }
     }
-    if (st + 1u < stages) stash(buf ^ 1u);  // last read a stage ago, before the barrier below
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < GW * NT; ++k)
+      xx[k] = __builtin_bit_cast(f16x8, at[((wm * MT + m) * STEPS + (u * WK + wk) * GW) * NT * kWave + k * kWave + lane]);
+  };
+  // Products of unit j (`words` and `scales` are its sub-group's), each block
+  // of rows beside the sum of the block before.
+  auto run_unit = [&](uint32_t j, const uint4 (&words)[NB], const float (&scales)[NB], const f16x8 (&xx)[GW * NT]) {
+    const uint32_t m = j % MT;
+    if (m == 0u) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        q[nb][0] = nibble_operand(words[nb].x), q[nb][1] = nibble_operand(words[nb].y);
+        if constexpr (GW == 4) q[nb][2] = nibble_operand(words[nb].z), q[nb][3] = nibble_operand(words[nb].w);
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t s = j * NB + nb, pm = (s + kUnits * NB - 1u) / NB % MT, pb = (s + NB - 1u) % NB;
+      f32x16& to = d[s % 2u];
+      const f32x16& from = d[(s + 1u) % 2u];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) to[i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < GW; ++k)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) to = Tile<32>::mfma(xx[k * NT + t], q[nb][k], to);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) total[pb][pm][i] = fmaf(before, from[i], total[pb][pm][i]);
+      before = scales[nb];
+    }
+  };
+  // A stage ends where its last unit's operands are read: its place is then
+  // filled anew, and the next stage read, before that unit's products. The
+  // wait leaves at most the RING - 2 stages after next outstanding: loads
+  // complete in order, so the next stage's are done, on every wavefront after
+  // the barrier; this wavefront's LDS reads are done as well.
+  auto arrive = [&](auto left) {
+    constexpr int LEFT = decltype(left)::value;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm(LEFT * kLoads));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto step = [&](uint4* at, const uint4* then, uint32_t st) {
+#pragma unroll
+    for (uint32_t j = 0; j < kUnits; ++j) {
+      uint4 words[NB];
+      float scales[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) words[nb] = w[nb], scales[nb] = scale[nb];
+      if (j + 1u < kUnits) {
+        load_unit(at, j + 1u, x[(j + 1u) % 2u]);
+      } else {
+        arrive(std::integral_constant<int, RING - 2>{});
+        issue(at, st + RING);
+        load_unit(then, 0u, x[(j + 1u) % 2u]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      run_unit(j, words, scales, x[j % 2u]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  arrive(std::integral_constant<int, RING - 1>{});
+  load_unit(l0, 0u, x[0]);
+  static_assert(kUnits % 2u == 0u, "units alternate between two sets of registers");
+  for (uint32_t st = 0; st < stages; st += RING) {
+    step(l0, l1, st);
+    step(l1, l2, st + 1u);
+    if constexpr (RING == 4) {
+      step(l2, l3, st + 2u);
+      step(l3, l0, st + 3u);
+    } else {
+      step(l2, l0, st + 2u);
+    }
   }
 #pragma unroll
+  for (int i = 0; i < 16; ++i) total[NB - 1][MT - 1][i] = fmaf(before, d[1][i], total[NB - 1][MT - 1][i]);
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // nothing is on its way into LDS when the workgroup ends or uses it anew
+  uint32_t nrow[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const uint32_t n = n0 + (wn * NB + nb) * 32u + row;
+    nrow[nb] = n < N ? n : N - 1u;
+  }
+  __syncthreads();  // the stages' places are free
+  if constexpr (WK > 1) {
+    // The wavefronts of a tile add up in the first's registers, in order.
+    static_assert(WK == 2, "one other");
+    static_assert(sizeof(float) * 16u * NB * MT * kWave * WM * WN <= sizeof(l0), "the sums fit a stage's place");
+    float* part = reinterpret_cast<float*>(l0) + (wave % (WM * WN)) * 16u * NB * MT * kWave;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (wk == 1u) part[((nb * MT + m) * 16 + i) * kWave + lane] = total[nb][m][i];
+    __syncthreads();
+    if (wk == 1u) return;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total[nb][m][i] += part[((nb * MT + m) * 16 + i) * kWave + lane];
+  }
+  // Outputs of 16 bits go through LDS (a place of the wavefront's own, in the
+  // second and third stages') and leave as 16 bytes a lane, whole lines where
+  // two lanes' halves of a line each would go out alone.
+  constexpr uint32_t kPitch = NB * 32u + 8u;  // elements of a token's row there
+  static_assert((WM * WN + 1u) / 2u * 32u * kPitch * 2u <= sizeof(l1), "the outputs fit two stages' places");
+  uint16_t* mine = reinterpret_cast<uint16_t*>(wave % 2u ? l1 : l2) + wave % (WM * WN) / 2u * 32u * kPitch;
+  const uint32_t nw = n0 + wn * NB * 32u;  // the wavefront's first row of W
+#pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const uint32_t tile = tile0 + wm * MT + m;
-    if (tile >= mp.tiles) break;
+    const uint32_t local = (wm * MT + m) * 32u, tile = tile0 + wm * MT + m;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int e = p.in.exps[tile * 32u + Tile<32>::row(lane, i)];
+      const int e = static_cast<int>(info[1][local + Tile<32>::row(lane, i)]);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) total[nb][m][i] = ldexpf(total[nb][m][i], e);
     }
-    if (p.ad.count) {
-      // One product per adapter that the tile's tokens have, added to its own tokens' rows.
-      const uint32_t i = tile * 32u + row;
-      uint32_t a = 0, rank = 0;
-      if (i < p.tokens) rank = token_rank(p.ad, p.ids, mp.order ? mp.order[i] : i, a);
-      const float* v = p.in.v + static_cast<size_t>(i < p.tokens ? i : 0u) * p.in.vr + 8u * slot;
-      uint32_t left = static_cast<uint32_t>(__ballot(rank != 0u));
-      while (left) {
-        const int leader = __builtin_ctz(left);
-        const uint32_t aa = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a), leader));
-        const uint32_t rr = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), leader));
-        const uint32_t same = static_cast<uint32_t>(__ballot(rank != 0u && a == aa));
-        left &= ~same;
-        f32x16 e[NB];
+    // One product per adapter that the tile's tokens have, added to its own
+    // tokens' rows.
+    const uint32_t a = info[2][local + row], rank = info[3][local + row];
+    uint32_t left = static_cast<uint32_t>(__ballot(rank != 0u));
+    while (left) {
+      const int leader = __builtin_ctz(left);
+      const uint32_t aa = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a), leader));
+      const uint32_t rr = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), leader));
+      const uint32_t same = static_cast<uint32_t>(__ballot(rank != 0u && a == aa));
+      left &= ~same;
+      f32x16 e[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int k = 0; k < 16; ++k) e[nb][k] = 0.0f;
-        for (uint32_t j = 0; j < rr; j += 16u) {
-          float c[8];
-          load8<OSM_META_F32>(v, j, true, c);
-          bf16x8 vt[3];
-          split_terms(c, vt);
+        for (int k = 0; k < 16; ++k) e[nb][k] = 0.0f;
+      const __bf16* v = mp.many.v_frag + (static_cast<size_t>(tile < mp.tiles ? tile : 0u) * (p.in.vr / 16u) * 3u * kWave + lane) * 8u;
+      if (p.ad.dtype == OSM_META_BF16)
+        expand_tile<OSM_META_BF16, NB>(p, aa, rr, v, nrow, slot, e);
+      else if (p.ad.dtype == OSM_META_F16)
+        expand_tile<OSM_META_F16, NB>(p, aa, rr, v, nrow, slot, e);
+      else
+        expand_tile<OSM_META_F32, NB>(p, aa, rr, v, nrow, slot, e);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (p.ad.dtype == OSM_META_BF16) {
-              bf16x8 bt[1];
-              expand_operand(p, aa, nrow[nb], j + 8u * slot, rr, bt);
-              e[nb] = mfma_terms(vt, bt, e[nb]);
-            } else {
-              bf16x8 bt[3];
-              expand_operand(p, aa, nrow[nb], j + 8u * slot, rr, bt);
-              e[nb] = mfma_terms(vt, bt, e[nb]);
-            }
-          }
-        }
+      for (int k = 0; k < 16; ++k) {
+        const bool own = (same >> Tile<32>::row(lane, k)) & 1u;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const bool own = (same >> Tile<32>::row(lane, k)) & 1u;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) total[nb][m][k] += own ? e[nb][k] : 0.0f;
-        }
+        for (int nb = 0; nb < NB; ++nb) total[nb][m][k] += own ? e[nb][k] : 0.0f;
       }
     }
+    if (mp.y_wide && nw + NB * 32u <= N) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t o = tile * 32u + Tile<32>::row(lane, i);
-      if (o >= p.tokens) continue;
-      const size_t t = mp.order ? mp.order[o] : o;
+      for (int i = 0; i < 16; ++i)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t n = n0 + (wn * NB + nb) * 32u + row;
-        if (n < N) store_out(p.y, p.y_dtype, t * p.y_stride + n, total[nb][m][i]);
+        for (int nb = 0; nb < NB; ++nb) {
+          const float v = total[nb][m][i];
+          mine[Tile<32>::row(lane, i) * kPitch + nb * 32u + row] =
+              p.y_dtype == OSM_META_BF16 ? __builtin_bit_cast(uint16_t, static_cast<__bf16>(v))
+                                         : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      constexpr uint32_t kPieces = NB * 4u;  // 16-byte pieces of a token's row
+#pragma unroll
+      for (uint32_t i = 0; i < 32u * kPieces / kWave; ++i) {
+        const uint32_t r = (i * kWave + lane) / kPieces, c = (i * kWave + lane) % kPieces;
+        const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kPitch + c * 8u);
+        if (tile * 32u + r < p.tokens)
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + info[0][local + r] * p.y_stride + nw + c * 8u) = v;
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();  // the next tile's outputs take the same place
+      continue;
     }
+    auto store = [&](auto put) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t r = Tile<32>::row(lane, i);
+        const size_t o = info[0][local + r] * p.y_stride;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const uint32_t n = nw + nb * 32u + row;
+          if (tile * 32u + r < p.tokens && n < N) put(o + n, total[nb][m][i]);
+        }
+      }
+    };
+    if (p.y_dtype == OSM_META_F32)
+      store([&](size_t o, float v) { static_cast<float*>(p.y)[o] = v; });
+    else if (p.y_dtype == OSM_META_BF16)
+      store([&](size_t o, float v) { static_cast<__bf16*>(p.y)[o] = static_cast<__bf16>(v); });
+    else
+      store([&](size_t o, float v) { static_cast<_Float16*>(p.y)[o] = static_cast<_Float16>(v); });
   }
 }
 
@@ -1153,8 +1370,8 @@ Plan plan_of(const osmd_project_args& a) {
       p.kgs = (subs + 15u) / 16u;
       p.bias_terms = a.w.meta_dtype == OSM_META_BF16 ? 1u : a.w.meta_dtype == OSM_META_F16 ? 2u : 3u;
       p.sums = take(static_cast<size_t>(p.rows) * p.kgs * 16u * kSumTerms * 2u);
-      p.scales = take(static_cast<size_t>(subs) * N * 4u);
-      p.biases = take(static_cast<size_t>(round_up(N, 32u)) * p.kgs * 16u * p.bias_terms * 2u);
+      p.scales = take((static_cast<size_t>(subs) + 1u) * round_up(N, 256u) * 4u);
+      p.biases = take(static_cast<size_t>(round_up(N, 256u)) * p.kgs * 16u * p.bias_terms * 2u);
       p.sort = a.adapters.count > 1u && a.adapters.count <= OSMD_GROUP_MAX_BUCKETS;
       if (p.sort) {
         p.order = take(static_cast<size_t>(a.tokens) * 4u);
@@ -1162,7 +1379,8 @@ Plan plan_of(const osmd_project_args& a) {
       }
     }
   }
-  p.v = take(static_cast<size_t>(a.tokens) * p.vr * sizeof(float));
+  // v: fp32 rows, or the three bf16 terms of whole tiles.
+  p.v = take(p.path == Path::kMany ? static_cast<size_t>(p.rows) * p.vr * 6u : static_cast<size_t>(a.tokens) * p.vr * sizeof(float));
   p.total = at;
   return p;
 }
@@ -1224,11 +1442,13 @@ int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipSt
   ManyParams mp{};
   mp.p = project_params(a, pl, work);
   mp.tiles = pl.rows / 32u;
-  mp.bias_terms = pl.bias_terms;
+  mp.y_wide = a.y_dtype != OSM_META_F32 && wide_rows(a.y, a.y_stride, a.y_dtype) ? 1u : 0u;
   mp.many.sum_frag = reinterpret_cast<__bf16*>(work + pl.sums);
   mp.many.scales = reinterpret_cast<float*>(work + pl.scales);
   mp.many.bias_frag = reinterpret_cast<__bf16*>(work + pl.biases);
   mp.many.kgs = pl.kgs;
+  mp.many.scale_row = round_up(a.w.out_dim, 256u);
+  mp.many.v_frag = reinterpret_cast<__bf16*>(work + pl.v);
   int r = 0;
   if (pl.sort) {
     // Tokens by adapter: a tile then holds one, or the few whose runs meet in it.
@@ -1251,54 +1471,53 @@ int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipSt
   pp.groups = mp.p.groups;
   pp.per_group = mp.p.per_group;
   pp.subs = a.w.packed_cols * 8u / pl.sub_cols;
-  // 32 or 64 threads a row while they hold it in registers, else the workgroup.
-  const uint32_t per_row = a.w.packed_cols <= 256u ? 32u : a.w.packed_cols <= 512u ? 64u : 256u;
-  pp.x_blocks = pl.rows * per_row / 256u;
-  const uint32_t meta_blocks = (a.w.out_dim + 31u) / 32u * pl.kgs;
+  // A wavefront a row while it holds the row in registers, else the workgroup.
+  const bool wave_rows = a.w.packed_cols <= 512u;
+  pp.x_blocks = wave_rows ? pl.rows / kShrinkManyWaves : pl.rows;
+  const uint32_t meta_blocks = round_up(a.w.out_dim, 256u) / 32u * pl.kgs;
+  const uint32_t ranks = pl.vr <= 16u ? 16u : 64u;  // of a shrinking workgroup
+  pp.shrink_blocks = a.adapters.count ? (a.tokens + 15u) / 16u * ((pl.vr + ranks - 1u) / ranks) : 0u;
+  pp.s = ShrinkManyParams{shrink_params(a, pl, work), mp.order, mp.many.v_frag};
   r = by_dtype(a.x_dtype, [&](auto xt) {
-    return by_dtype(a.w.meta_dtype, [&](auto meta) {
-      constexpr int X = decltype(xt)::value, M = decltype(meta)::value;
-      auto go = [&](auto kernel) { kernel<<<pp.x_blocks + meta_blocks, 256, 0, st>>>(pp); };
-      if (per_row == 32u)
-        go(prepare_many_kernel<X, GW, M, 32>);
-      else if (per_row == 64u)
-        go(prepare_many_kernel<X, GW, M, 64>);
-      else
-        go(prepare_many_kernel<X, GW, M, 256>);
-      return launch_status();
+    return by_dtype(a.adapters.dtype, [&](auto at) {
+      constexpr int X = decltype(xt)::value, A = decltype(at)::value;
+      auto go = [&](auto kernel) {
+        kernel<<<pp.shrink_blocks + pp.x_blocks + meta_blocks, kPrepareThreads, 0, st>>>(pp);
+        return launch_status();
+      };
+      if (ranks == 16u)
+        return wave_rows ? go(prepare_many_kernel<X, GW, 64, A, 1>) : go(prepare_many_kernel<X, GW, kPrepareThreads, A, 1>);
+      return wave_rows ? go(prepare_many_kernel<X, GW, 64, A, 4>) : go(prepare_many_kernel<X, GW, kPrepareThreads, A, 4>);
     });
   });
   if (r != 0) return r;
-  if (a.adapters.count) {
-    ShrinkManyParams sp{shrink_params(a, pl, work), mp.order};
-    r = by_dtype(a.x_dtype, [&](auto xt) {
-      return by_dtype(a.adapters.dtype, [&](auto at) {
-        constexpr int X = decltype(xt)::value, A = decltype(at)::value;
-        auto go = [&](auto kernel, uint32_t ranks) {
-          kernel<<<dim3((a.tokens + 15u) / 16u, (pl.vr + ranks - 1u) / ranks), kShrinkManyWaves * kWave, 0, st>>>(sp);
-        };
-        if (pl.vr <= 16u)
-          go(shrink_many_kernel<X, A, 1>, 16u);
-        else if (pl.vr <= 32u)
-          go(shrink_many_kernel<X, A, 2>, 32u);
-        else
-          go(shrink_many_kernel<X, A, 4>, 64u);
-        return launch_status();
-      });
-    });
-    if (r != 0) return r;
-  }
   auto go = [&](auto kernel, uint32_t tiles, uint32_t rows, uint32_t threads) {
     const uint32_t grid = (mp.tiles + tiles - 1u) / tiles * ((a.w.out_dim + rows - 1u) / rows);
     kernel<<<grid, threads, 0, st>>>(mp);
     return launch_status();
   };
-  const bool big = (mp.tiles + 3u) / 4u * ((a.w.out_dim + 255u) / 256u) >= 256u;
-  if (pl.terms == 2u)
-    return big ? go(project_many_kernel<2, 2, 2, 2, 4, GW, 64>, 4u, 256u, 512u)
-               : go(project_many_kernel<2, 1, 1, 2, 4, GW, 128>, 2u, 128u, 512u);
-  return big ? go(project_many_kernel<1, 2, 2, 2, 4, GW, 128>, 4u, 256u, 512u)
-             : go(project_many_kernel<1, 1, 1, 2, 4, GW, 256>, 2u, 128u, 512u);
+  // The tile with the least time expected: microseconds of a round of
+  // workgroups at 2,048 columns (the others' in proportion) times the rounds.
+  // One term, tiles of 64 x 128 / 128 x 128 / 128 x 256, measured: 512 tokens
+  // through 4,096 rows 16 / 26 / 33, 1,024: 29 / 29 / 36, 2,048: 59 / 45 / 42.
+  // Two terms, 32 x 128 / 128 x 256: 31 / 74, 59 / 76, 130 / 94.
+  auto groups = [&](uint32_t tiles, uint32_t rows) {
+    return (mp.tiles + tiles - 1u) / tiles * ((a.w.out_dim + rows - 1u) / rows);
+  };
+  return by_dtype(a.w.meta_dtype, [&](auto meta) {
+    constexpr int M = decltype(meta)::value;
+    if (pl.terms == 2u) {
+      if ((groups(1u, 128u) + 255u) / 256u * 15u <= (groups(4u, 256u) + 255u) / 256u * 92u)
+        return go(project_many_kernel<M, 2, 1, 1, 1, 4, 2, GW, 256, 3>, 1u, 128u, 512u);
+      return go(project_many_kernel<M, 2, 2, 2, 2, 4, 1, GW, 64, 3>, 4u, 256u, 512u);
+    }
+    const uint32_t small = (groups(2u, 128u) + 255u) / 256u * 15u;
+    const uint32_t middle = groups(4u, 128u) <= 256u ? 26u : (groups(4u, 128u) + 511u) / 512u * 45u;
+    const uint32_t large = (groups(4u, 256u) + 255u) / 256u * 41u;
+    if (small <= middle && small <= large) return go(project_many_kernel<M, 1, 1, 1, 2, 4, 1, GW, 128, 4>, 2u, 128u, 512u);
+    if (middle <= large) return go(project_many_kernel<M, 1, 2, 2, 2, 2, 1, GW, 64, 3>, 4u, 128u, 256u);
+    return go(project_many_kernel<M, 1, 2, 2, 2, 4, 1, GW, 64, 3>, 4u, 256u, 512u);
+  });
 }
 
 int launch_vec(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStream_t st) {
