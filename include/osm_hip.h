@@ -234,7 +234,8 @@ int osm_route_experts(osm_context ctx, const osm_route_rule* rule, const void* l
  * key 1, ..., then those whose key is outside [0, buckets), each in row order;
  * offsets [buckets + 1] say where each key's rows start (the last entry: where
  * the rows outside do). Groups (token, expert) pairs by expert, or a batch's
- * tokens by adapter. buckets in [1, 65535]. */
+ * tokens by adapter. buckets in [1, 65535]. More than 16,384 rows are grouped
+ * in the context's shared workspace (see osm_q4_project). */
 int osm_group_rows(osm_context ctx, const int32_t* keys_dev, uint32_t rows, uint32_t buckets,
                    uint32_t* offsets_dev, uint32_t* order_dev);
 /* Low-rank adapters of one projection, in device memory of the caller's.

@@ -231,10 +231,12 @@ int osmd_moe_select_rule(const osmd_moe_args* a, osmd_stream s);
 
 /* Rows grouped by key, stable: order [rows] holds the rows of key 0, of key
  * 1, ..., then those whose key is outside [0, buckets); offsets [buckets + 1]
- * where each starts (the last: where the rows outside start). */
+ * where each starts (the last: where the rows outside start). workspace:
+ * osmd_group_rows_workspace bytes (0 for few rows). */
 #define OSMD_GROUP_MAX_BUCKETS 65535u
+size_t osmd_group_rows_workspace(uint32_t rows, uint32_t buckets);
 int osmd_group_rows(const int32_t* keys, uint32_t rows, uint32_t buckets, uint32_t* offsets, uint32_t* order,
-                    osmd_stream s);
+                    void* workspace, osmd_stream s);
 
 /* y = W x + scale_a B_a (A_a x) for tokens rows, a = adapter_ids[token] (none
  * outside [0, count)). v [tokens, max_rank] fp32 scratch (adapters only). */

@@ -1336,7 +1336,7 @@ struct Plan {
   Path path;
   bool sort;
   uint32_t sub_cols, tile, rows, terms, vr, kgs, bias_terms;
-  size_t frag, sums, exps, scales, biases, order, offsets, v, total;  // workspace offsets
+  size_t frag, sums, exps, scales, biases, order, offsets, counts, v, total;  // workspace offsets
 };
 Plan plan_of(const osmd_project_args& a) {
   Plan p{};
@@ -1376,6 +1376,7 @@ Plan plan_of(const osmd_project_args& a) {
       if (p.sort) {
         p.order = take(static_cast<size_t>(a.tokens) * 4u);
         p.offsets = take((static_cast<size_t>(a.adapters.count) + 1u) * 4u);
+        p.counts = take(osmd_group_rows_workspace(a.tokens, a.adapters.count));
       }
     }
   }
@@ -1453,7 +1454,8 @@ int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipSt
   if (pl.sort) {
     // Tokens by adapter: a tile then holds one, or the few whose runs meet in it.
     uint32_t* order = reinterpret_cast<uint32_t*>(work + pl.order);
-    r = osmd_group_rows(a.adapter_ids, a.tokens, a.adapters.count, reinterpret_cast<uint32_t*>(work + pl.offsets), order, st);
+    r = osmd_group_rows(a.adapter_ids, a.tokens, a.adapters.count, reinterpret_cast<uint32_t*>(work + pl.offsets), order, work + pl.counts,
+                        st);
     if (r != 0) return r;
     mp.order = order;
   }

@@ -25,6 +25,24 @@ HipDispatchResult refused(std::string why) {
   return r;
 }
 
+// `bytes` of the context's shared workspace, which does not grow while a
+// capture is recording on its stream; nullptr with the reason in *why.
+void* workspace(HipComputeContext& context, std::size_t bytes, const char* what, std::string* why) {
+  int rc = 0;
+  if (bytes > context.shared_workspace_bytes()) {
+    int capturing = 0;
+    rc = osmd_stream_capturing(context.stream(), &capturing);
+    if (rc != 0) return *why = hip_error((std::string(what) + ": stream query failed").c_str(), rc), nullptr;
+    if (capturing)
+      return *why = std::string(what) + ": the context's workspace is too small for this call and cannot grow during a "
+                                        "capture; make the call once before it",
+             nullptr;
+  }
+  void* p = context.shared_workspace(bytes, &rc);
+  if (p == nullptr) *why = hip_error((std::string(what) + ": workspace allocation failed").c_str(), rc);
+  return p;
+}
+
 HipDispatchResult enqueued(int rc, const char* failed, const char* done) {
   HipDispatchResult r;
   r.executed = rc == 0;
@@ -99,8 +117,11 @@ HipDispatchResult run_hip_group_rows(HipComputeContext& context, const std::int3
       return refused("row grouping: an array is not aligned to its elements");
     std::string d;
     if (!context.activate(&d)) return refused(d);
-    return enqueued(osmd_group_rows(keys, rows, buckets, offsets, order, context.stream()), "row grouping launch failed",
-                    "HIP row grouping enqueued.");
+    const std::size_t bytes = osmd_group_rows_workspace(rows, buckets);
+    void* work = bytes != 0U ? workspace(context, bytes, "row grouping", &d) : nullptr;
+    if (bytes != 0U && work == nullptr) return refused(d);
+    return enqueued(osmd_group_rows(keys, rows, buckets, offsets, order, work, context.stream()),
+                    "row grouping launch failed", "HIP row grouping enqueued.");
   } catch (...) {
     return HipDispatchResult{};
   }
@@ -152,20 +173,8 @@ HipDispatchResult run_hip_q4_project(HipComputeContext& context, const HipQ4Proj
     if ((N + 3U) / 4U * ((tokens + 3U) / 4U) > (std::size_t{1} << 30))
       return refused("Q4 projection: out_dim x tokens exceeds the kernels' grids; split the call");
     const std::size_t bytes = osmd_q4_project_workspace(&a);
-    void* work = nullptr;
-    if (bytes != 0U) {
-      if (bytes > context.shared_workspace_bytes()) {
-        int capturing = 0;
-        int rc = osmd_stream_capturing(context.stream(), &capturing);
-        if (rc != 0) return refused(hip_error("Q4 projection: stream query failed", rc));
-        if (capturing)
-          return refused("Q4 projection: the context's workspace is too small for this call and cannot grow during a "
-                         "capture; make the call once before it");
-      }
-      int rc = 0;
-      work = context.shared_workspace(bytes, &rc);
-      if (work == nullptr) return refused(hip_error("Q4 projection workspace allocation failed", rc));
-    }
+    void* work = bytes != 0U ? workspace(context, bytes, "Q4 projection", &d) : nullptr;
+    if (bytes != 0U && work == nullptr) return refused(d);
     return enqueued(osmd_q4_project(&a, work, context.stream()), "Q4 projection launch failed",
                     "HIP Q4 projection enqueued.");
   } catch (...) {

@@ -29,8 +29,8 @@ def expected(keys, buckets):
     return np.cumsum(counts) - counts, np.argsort(b, kind="stable")
 
 
-@pytest.mark.parametrize("n", [0, 1, 63, 64, 65, 1000, 1025, 4097, 81920, 300007])
-@pytest.mark.parametrize("buckets", [1, 2, 7, 255, 256, 512, 1000, 65535])
+@pytest.mark.parametrize("n", [0, 1, 63, 64, 65, 1000, 1025, 4097, 16384, 16385, 81920, 300007, 1100003])
+@pytest.mark.parametrize("buckets", [1, 2, 7, 255, 256, 512, 1000, 2047, 2048, 65535])
 def test_matches_stable_sort(ctx, n, buckets):
     rng = np.random.default_rng(n + buckets)
     print(f"[group] n={n} buckets={buckets}", flush=True)
