@@ -137,11 +137,28 @@ struct PrepareParams {
   Prepared out;
 };
 
-struct ManyPrepared;
+constexpr int kSumTerms = 3;
 
-template <int TERMS>
-__device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v);
-__device__ __forceinline__ uint32_t many_columns(const ManyPrepared& m);
+// What the tiled kernel reads besides the fragments.
+struct ManyPrepared {
+  __bf16* sum_frag;   // [tile][16 sub-groups][term][64][8]
+  float* scales;      // [sub-group][row of W, scale_row apart], then a row of zeros
+  uint32_t scale_row;
+  __bf16* bias_frag;  // [32 rows][16 sub-groups][term][64][8]
+  uint32_t kgs;       // runs of 16 sub-groups
+  __bf16* v_frag;     // [tile][16 rank rows][term][64][8]: v, scale_a A_a x
+};
+
+// The sum of a sub-group of a token as bf16 terms, each the nearest to what is left.
+__device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v) {
+  const uint32_t lane = sub % 16u / 8u * 32u + row;
+#pragma unroll
+  for (int t = 0; t < kSumTerms; ++t) {
+    const __bf16 b = static_cast<__bf16>(v);
+    m.sum_frag[(((static_cast<size_t>(tile) * m.kgs + sub / 16u) * kSumTerms + t) * kWave + lane) * 8u + sub % 8u] = b;
+    v -= static_cast<float>(b);
+  }
+}
 
 // TPT threads a row, of a workgroup's THREADS.
 template <int XT, int R, int GW, int TPT, int THREADS = 256, bool MANY = false>
@@ -191,34 +208,34 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
     if (p.words > kKeep * TPT) batch(w0);
 #pragma unroll
     for (uint32_t u = 0; u < kKeep; ++u) {
-    const uint32_t w = w0 + u * TPT;
-    if (w >= p.words) break;  // whole groups of GWS lanes leave together (words is a multiple of GWS)
-    float sum = 0.0f;
-    f16x8 hi, lo;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      constexpr int nibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-      const float s = live ? ldexpf(keep[u].get(nibble[k]), e) : 0.0f;
-      sum += s;
-      const float o = (nibble[k] & 1) ? s * 0.0625f : s;
-      hi[k] = static_cast<_Float16>(o);
-      if constexpr (NT == 2) lo[k] = static_cast<_Float16>(o - static_cast<float>(hi[k]));
-    }
-    const uint32_t sub = w / GWS, iw = w % GWS;
-    const uint32_t lane = iw / GW * R + row % R, step = sub * GW + iw % GW;
-    _Float16* f = p.out.frag + ((static_cast<size_t>(tile) * steps + step) * NT * kWave + lane) * 8u;
-    *reinterpret_cast<f16x8*>(f) = hi;
-    if constexpr (NT == 2) *reinterpret_cast<f16x8*>(f + kWave * 8u) = lo;
-    sum = row_sum<GWS < 16 ? GWS : 16>(sum);
-    if constexpr (MANY) {
-      if (iw == 0) {
-        store_sum<3>(*many, tile, sub, row % R, sum * 0x1p-24f);
-        if (sub + 1u == subs)
-          for (uint32_t z = subs; z < many_columns(*many); ++z) store_sum<3>(*many, tile, z, row % R, 0.0f);
+      const uint32_t w = w0 + u * TPT;
+      if (w >= p.words) break;  // whole groups of GWS lanes leave together (words is a multiple of GWS)
+      float sum = 0.0f;
+      f16x8 hi, lo;
+  #pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        constexpr int nibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+        const float s = live ? ldexpf(keep[u].get(nibble[k]), e) : 0.0f;
+        sum += s;
+        const float o = (nibble[k] & 1) ? s * 0.0625f : s;
+        hi[k] = static_cast<_Float16>(o);
+        if constexpr (NT == 2) lo[k] = static_cast<_Float16>(o - static_cast<float>(hi[k]));
       }
-    } else {
-      if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
-    }
+      const uint32_t sub = w / GWS, iw = w % GWS;
+      const uint32_t lane = iw / GW * R + row % R, step = sub * GW + iw % GW;
+      _Float16* f = p.out.frag + ((static_cast<size_t>(tile) * steps + step) * NT * kWave + lane) * 8u;
+      *reinterpret_cast<f16x8*>(f) = hi;
+      if constexpr (NT == 2) *reinterpret_cast<f16x8*>(f + kWave * 8u) = lo;
+      sum = row_sum<GWS < 16 ? GWS : 16>(sum);
+      if constexpr (MANY) {
+        if (iw == 0) {
+          store_sum(*many, tile, sub, row % R, sum * 0x1p-24f);
+          if (sub + 1u == subs)
+            for (uint32_t z = subs; z < many->kgs * 16u; ++z) store_sum(*many, tile, z, row % R, 0.0f);
+        }
+      } else {
+        if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
+      }
     }
   }
 }
@@ -244,12 +261,23 @@ __device__ __forceinline__ void shrink_rows(const ShrinkParams& p, uint32_t bloc
   float s = 0.0f;
   if (j < rank) {
     const size_t xo = t * p.stride, ao = (static_cast<size_t>(a) * p.ad.max_rank + j) * p.words * 8u;
-    for (uint32_t w = lane; w < p.words; w += kWave) {
-      float x[8], c[8];
-      load8<XT>(p.x, xo + 8u * w, p.x_wide, x);
-      load8<AT>(p.ad.a, ao + 8u * w, p.a_wide, c);
+    constexpr uint32_t kAhead = 4;  // pieces of 8 columns in flight
+    for (uint32_t w0 = lane; w0 < p.words; w0 += kAhead * kWave) {
+      Raw8<XT> x[kAhead];
+      Raw8<AT> c[kAhead];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s = fmaf(x[k], c[k], s);
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        const uint32_t w = w0 + u * kWave < p.words ? w0 + u * kWave : w0;
+        load_raw8<XT>(p.x, xo + 8u * w, p.x_wide, x[u]);
+        load_raw8<AT>(p.ad.a, ao + 8u * w, p.a_wide, c[u]);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        float d = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d = fmaf(x[u].get(k), c[u].get(k), d);
+        s += w0 + u * kWave < p.words ? d : 0.0f;
+      }
     }
     s = wave_sum(s);
     if (p.ad.scales) s *= p.ad.scales[a];
@@ -528,7 +556,7 @@ __global__ __launch_bounds__(kFewWaves* kWave, 4) void project_few_kernel(Projec
 }
 
 // ---- one to four tokens ----------------------------------------------------------
-// A wavefront takes kVecRows rows of W; a lane holds 32 consecutive columns of
+// A wavefront takes ROWS rows of W; a lane holds 32 consecutive columns of
 // each token in registers (a chunk, within one quantisation group) and the
 // chunk's sum for the bias. No preparation: one launch, after the shrink.
 constexpr int kVecWaves = 4;
@@ -608,17 +636,15 @@ __global__ __launch_bounds__(kVecWaves* kWave) void project_vec_kernel(VecParams
 
 // ---- many tokens -------------------------------------------------------------------
 // Tiles of 32 x 32 outputs, W unpacked in registers and used for MT tiles of
-// tokens; the tokens' fragments and the packed words are staged through LDS,
-// the next stage's on their way in registers while one computes. Per output
-// and sub-group of 64 columns that is 64 products on the matrix cores against
-// one FMA (the scale) and 64 / (32 MT) unpacked nibbles on the vector units;
-// the biases, a product of [tokens, sub-groups] by [sub-groups, rows], are on
-// the matrix cores too. Their factors are split into bf16 terms (the sums into
+// tokens; the tokens' fragments and the packed words go straight from memory
+// into LDS, a ring of stages ahead of the one that computes. Per output and
+// sub-group of 64 columns that is 64 products on the matrix cores against one
+// FMA (the scale) and 64 / (32 MT) unpacked nibbles on the vector units; the
+// biases, a product of [tokens, sub-groups] by [sub-groups, rows], are on the
+// matrix cores too. Their factors are split into bf16 terms (the sums into
 // three; a bias into one, two or three by its type), products below 2^-24 of
 // the whole left out. Before the main launch one prepares x (as above), the
 // scales transposed to [sub-group][row] and the biases as operands.
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
 template <int AT>
 constexpr int kTerms = AT == OSM_META_BF16 ? 1 : AT == OSM_META_F16 ? 2 : 3;  // exact in that many bf16 terms
 
@@ -668,30 +694,7 @@ __device__ __forceinline__ void raw_terms(const Raw8<T>& r, bf16x8 (&t)[NT]) {
   }
 }
 
-constexpr int kSumTerms = 3;
-
-struct ManyPrepared {
-  __bf16* sum_frag;   // [tile][16 sub-groups][term][64][8]
-  float* scales;      // [sub-group][row of W, scale_row apart], then a row of zeros
-  uint32_t scale_row;
-  __bf16* bias_frag;  // [32 rows][16 sub-groups][term][64][8]
-  uint32_t kgs;       // runs of 16 sub-groups
-  __bf16* v_frag;     // [tile][16 rank rows][term][64][8]: v, scale_a A_a x
-};
-
-__device__ __forceinline__ uint32_t many_columns(const ManyPrepared& m) { return m.kgs * 16u; }
 __device__ __forceinline__ bf16x8 load_bf16(const __bf16* p) { return __builtin_bit_cast(bf16x8, ldg<u32x4>(p)); }
-
-template <int TERMS>
-__device__ __forceinline__ void store_sum(const ManyPrepared& m, uint32_t tile, uint32_t sub, uint32_t row, float v) {
-  const uint32_t lane = sub % 16u / 8u * 32u + row;
-#pragma unroll
-  for (int t = 0; t < TERMS; ++t) {
-    const __bf16 b = static_cast<__bf16>(v);
-    m.sum_frag[(((static_cast<size_t>(tile) * m.kgs + sub / 16u) * TERMS + t) * kWave + lane) * 8u + sub % 8u] = b;
-    v -= static_cast<float>(b);
-  }
-}
 
 // Scales and biases of W for sub-groups of which `per_group` make a group: a
 // workgroup takes 16 sub-groups of 32 rows; what lies past the last is zero.
@@ -1275,40 +1278,42 @@ constexpr uint32_t kAnyTokens = 4;
 template <int META, int XT>
 __global__ __launch_bounds__(kAnyWaves* kWave) void project_any_kernel(osmd_project_args p, const float* __restrict__ v,
                                                                        uint32_t vr) {
-  const uint32_t N = p.w.out_dim, blocks = (N + kAnyWaves - 1u) / kAnyWaves;
+  const uint32_t N = p.w.out_dim;
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t n = blockIdx.x % blocks * kAnyWaves + wave, t0 = blockIdx.x / blocks * kAnyTokens;
+  const uint32_t n = blockIdx.x * kAnyWaves + wave;
   if (n >= N) return;
   const uint32_t words = p.w.packed_cols, G = p.w.group, groups = words * 8u / G;
-  float acc[kAnyTokens] = {};
-  size_t xo[kAnyTokens];
+  for (uint32_t t0 = blockIdx.y * kAnyTokens; t0 < p.tokens; t0 += gridDim.y * kAnyTokens) {
+    float acc[kAnyTokens] = {};
+    size_t xo[kAnyTokens];
 #pragma unroll
-  for (uint32_t i = 0; i < kAnyTokens; ++i) xo[i] = (t0 + i < p.tokens ? t0 + i : t0) * p.x_stride;
-  for (uint32_t w = lane; w < words; w += kWave) {
-    const uint32_t word = p.w.packed[static_cast<size_t>(n) * words + w];
-    for (uint32_t j = 0; j < 8u; ++j) {
-      const uint32_t c = 8u * w + j;
-      const size_t g = static_cast<size_t>(n) * groups + c / G;
-      const float q = static_cast<float>((word >> (4u * j)) & 15u);
-      const float value = fmaf(meta_at<META>(p.w.scales, g), q, meta_at<META>(p.w.biases, g));
+    for (uint32_t i = 0; i < kAnyTokens; ++i) xo[i] = (t0 + i < p.tokens ? t0 + i : t0) * p.x_stride;
+    for (uint32_t w = lane; w < words; w += kWave) {
+      const uint32_t word = p.w.packed[static_cast<size_t>(n) * words + w];
+      for (uint32_t j = 0; j < 8u; ++j) {
+        const uint32_t c = 8u * w + j;
+        const size_t g = static_cast<size_t>(n) * groups + c / G;
+        const float q = static_cast<float>((word >> (4u * j)) & 15u);
+        const float value = fmaf(meta_at<META>(p.w.scales, g), q, meta_at<META>(p.w.biases, g));
 #pragma unroll
-      for (uint32_t i = 0; i < kAnyTokens; ++i) acc[i] = fmaf(value, meta_at<XT>(p.x, xo[i] + c), acc[i]);
+        for (uint32_t i = 0; i < kAnyTokens; ++i) acc[i] = fmaf(value, meta_at<XT>(p.x, xo[i] + c), acc[i]);
+      }
     }
-  }
-  for (uint32_t i = 0; i < kAnyTokens && t0 + i < p.tokens; ++i) {
-    const uint32_t t = t0 + i, R = p.adapters.max_rank;
-    uint32_t a = 0;
-    const uint32_t rank = token_rank(p.adapters, p.adapter_ids, t, a);
-    float d = 0.0f;
-    for (uint32_t j = lane; j < rank; j += kWave) {
-      const size_t o = (static_cast<size_t>(a) * N + n) * R + j;
-      const float b = p.adapters.dtype == OSM_META_F32    ? meta_at<OSM_META_F32>(p.adapters.b, o)
-                      : p.adapters.dtype == OSM_META_BF16 ? meta_at<OSM_META_BF16>(p.adapters.b, o)
-                                                          : meta_at<OSM_META_F16>(p.adapters.b, o);
-      d = fmaf(b, v[static_cast<size_t>(t) * vr + j], d);
+    for (uint32_t i = 0; i < kAnyTokens && t0 + i < p.tokens; ++i) {
+      const uint32_t t = t0 + i, R = p.adapters.max_rank;
+      uint32_t a = 0;
+      const uint32_t rank = token_rank(p.adapters, p.adapter_ids, t, a);
+      float d = 0.0f;
+      for (uint32_t j = lane; j < rank; j += kWave) {
+        const size_t o = (static_cast<size_t>(a) * N + n) * R + j;
+        const float b = p.adapters.dtype == OSM_META_F32    ? meta_at<OSM_META_F32>(p.adapters.b, o)
+                        : p.adapters.dtype == OSM_META_BF16 ? meta_at<OSM_META_BF16>(p.adapters.b, o)
+                                                            : meta_at<OSM_META_F16>(p.adapters.b, o);
+        d = fmaf(b, v[static_cast<size_t>(t) * vr + j], d);
+      }
+      const float y = wave_sum(acc[i] + d);
+      if (lane == 0) store_out(p.y, p.y_dtype, t * p.y_stride + n, y);
     }
-    const float y = wave_sum(acc[i] + d);
-    if (lane == 0) store_out(p.y, p.y_dtype, t * p.y_stride + n, y);
   }
 }
 
@@ -1610,7 +1615,7 @@ int osmd_q4_project(const osmd_project_args* a, void* workspace, osmd_stream s) 
   return by_dtype(a->w.meta_dtype, [&](auto meta) {
     return by_dtype(a->x_dtype, [&](auto xt) {
       project_any_kernel<decltype(meta)::value, decltype(xt)::value>
-          <<<blocks * tiles, kAnyWaves * kWave, 0, st>>>(*a, v, pl.vr);
+          <<<dim3(blocks, tiles < 65535u ? tiles : 65535u), kAnyWaves * kWave, 0, st>>>(*a, v, pl.vr);
       return launch_status();
     });
   });

@@ -133,6 +133,23 @@ def test_matches_float64(ctx, T, N, K, group, x):
     Problem(ctx, T, N, K, group, meta, x, y=F32, count=5, rank=16, adapter=adapter).check()
 
 
+# Enough tokens and rows for the larger tiles, whole and ragged, over few columns.
+@pytest.mark.parametrize("T,N,K,group", [(1000, 4090, 160, 32), (1024, 4096, 320, 64), (2040, 4095, 96, 32), (2048, 4096, 448, 64)])
+@pytest.mark.parametrize("x", [F32, F16, BF16])
+def test_large_tiles(ctx, T, N, K, group, x):
+    print(f"[project] T={T} N={N} K={K} group={group} x={x}", flush=True)
+    for meta in (F32, F16, BF16):
+        Problem(ctx, T, N, K, group, meta, x, count=5 if meta == BF16 else 0, rank=24, ragged=True, y_pad=8 * (meta == F16)).check()
+
+
+def test_more_adapters_than_are_sorted(ctx):
+    for x in (F32, BF16):
+        for T in (3, 30, 130):
+            ids = np.arange(T) * 521 % 65537
+            ids[0], ids[T - 1], ids[1] = 65536, 65537, 65536
+            Problem(ctx, T, 40, 32, 32, BF16, x, count=65537, rank=1, ids=ids).check()
+
+
 @pytest.mark.parametrize("rank", [1, 3, 8, 16, 21, 64, 130, 256])
 @pytest.mark.parametrize("adapter", [F32, F16, BF16])
 @pytest.mark.parametrize("T", [1, 40, 200])
