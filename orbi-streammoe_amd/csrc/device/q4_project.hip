@@ -735,15 +735,29 @@ __device__ __forceinline__ void shrink_tile(const ShrinkManyParams& sp, uint32_t
   const ShrinkParams& p = sp.s;
   constexpr int NX = kTerms<XT>, NA = kTerms<AT>;
   // Steps in flight: within some 100 registers.
-  constexpr int kSteps = JB == 1 ? 6 : AT == OSM_META_F32 ? 2 : 4;
+  constexpr int kSteps = JB == 1 ? (XT == OSM_META_F32 || AT == OSM_META_F32 ? 6 : 8) : AT == OSM_META_F32 ? 2 : 4;
   __shared__ float part[kShrinkManyWaves][JB][4][kWave];
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, K = p.words * 8u;
+  const uint32_t lane = threadIdx.x % kWave, K = p.words * 8u;
+  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
   const uint32_t tiles = (p.tokens + 15u) / 16u, i0 = block % tiles * 16u, j0 = block / tiles * 16u * JB;
   const uint32_t i = i0 + lane % 16u, slot = lane / 16u;
   const uint32_t t = i < p.tokens ? (sp.order ? sp.order[i] : i) : 0u;
+  const size_t xo = t * p.stride + 8u * slot;
+  // The batch of x that the registers hold starts at column `held`; rows of
+  // one batch are read once for all adapters, and before those are known.
+  constexpr uint32_t kApart = kShrinkManyWaves * 32u;
+  Raw8<XT> x[kSteps];
+  uint32_t held = wave * 32u;
+  auto load_x = [&](uint32_t k0) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const uint32_t k = k0 + s * kApart;
+      load_raw8<XT>(p.x, xo + (k < K ? k : K - 32u), p.x_wide, x[s]);
+    }
+  };
+  load_x(held);
   uint32_t a = 0;
   const uint32_t rank = i < p.tokens ? token_rank(p.ad, p.ids, t, a) : 0u;
-  const size_t xo = t * p.stride + 8u * slot;
   uint64_t left = __ballot(rank != 0u) & 0xFFFFull;
   while (left) {
     const int leader = __builtin_ctzll(left);
@@ -751,6 +765,7 @@ __device__ __forceinline__ void shrink_tile(const ShrinkManyParams& sp, uint32_t
     const uint32_t rr = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), leader));
     const uint64_t same = __ballot(rank != 0u && a == aa) & 0xFFFFull;
     left &= ~same;
+    const float scale = p.ad.scales ? p.ad.scales[aa] : 1.0f;
     f32x4 acc[JB];
     size_t ao[JB];
 #pragma unroll
@@ -759,19 +774,19 @@ __device__ __forceinline__ void shrink_tile(const ShrinkManyParams& sp, uint32_t
       const uint32_t j = j0 + 16u * b + lane % 16u;  // rows past the rank repeat its last
       ao[b] = (static_cast<size_t>(aa) * p.ad.max_rank + (j < rr ? j : rr - 1u)) * K + 8u * slot;
     }
-    Raw8<XT> x[kSteps];
     Raw8<AT> c[kSteps][JB];
-    for (uint32_t k0 = wave * 32u; k0 < K; k0 += kSteps * kShrinkManyWaves * 32u) {
+    for (uint32_t k0 = wave * 32u; k0 < K; k0 += kSteps * kApart) {
+      if (held != k0) load_x(k0);
+      held = k0;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        const uint32_t at = k0 + s * kShrinkManyWaves * 32u, k = at < K ? at : k0;
-        load_raw8<XT>(p.x, xo + k, p.x_wide, x[s]);
+        const uint32_t k = k0 + s * kApart;
 #pragma unroll
-        for (int b = 0; b < JB; ++b) load_raw8<AT>(p.ad.a, ao[b] + k, p.a_wide, c[s][b]);
+        for (int b = 0; b < JB; ++b) load_raw8<AT>(p.ad.a, ao[b] + (k < K ? k : K - 32u), p.a_wide, c[s][b]);
       }
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        if (k0 + s * kShrinkManyWaves * 32u >= K) break;
+        if (k0 + s * kApart >= K) break;
         bf16x8 xt[NX];
         raw_terms(x[s], xt);
 #pragma unroll
@@ -787,7 +802,6 @@ __device__ __forceinline__ void shrink_tile(const ShrinkManyParams& sp, uint32_t
 #pragma unroll
       for (int e = 0; e < 4; ++e) part[wave][b][e][lane] = acc[b][e];
     __syncthreads();
-    const float scale = p.ad.scales ? p.ad.scales[aa] : 1.0f;
     for (uint32_t o = threadIdx.x; o < 16u * 16u * JB; o += kShrinkManyWaves * kWave) {
       const uint32_t r = o / (16u * JB), j = o % (16u * JB);
       if (!((same >> r) & 1u) || j0 + j >= p.vr) continue;
@@ -843,14 +857,16 @@ struct ManyParams {
 };
 
 // e += v of the tile's tokens times B_a of the rows nrow, over the a's rank;
-// the next step's loads are on their way while one computes.
+// the loads of kDeep steps are in flight together.
 template <int AT, int NB>
 __device__ __forceinline__ void expand_tile(const ProjectParams& p, uint32_t a, uint32_t rank, const __bf16* v_frag,
                                             const uint32_t (&nrow)[NB], uint32_t slot, f32x16 (&e)[NB]) {
   struct Step {
     bf16x8 v[3];
     Raw8<AT> b[NB];
-  } step[2];
+  };
+  constexpr uint32_t kDeep = AT == OSM_META_F32 ? 2 : 4;
+  Step step[kDeep];
   const uint32_t R = p.ad.max_rank;
   auto load = [&](Step& s, uint32_t j) {
 #pragma unroll
@@ -888,13 +904,13 @@ __device__ __forceinline__ void expand_tile(const ProjectParams& p, uint32_t a, 
       e[nb] = mfma_terms(s.v, bt, e[nb]);
     }
   };
-  load(step[0], 0u);
-  for (uint32_t j = 0; j < rank; j += 32u) {
-    if (j + 16u < rank) load(step[1], j + 16u);
-    compute(step[0], j);
-    if (j + 16u >= rank) break;
-    if (j + 32u < rank) load(step[0], j + 32u);
-    compute(step[1], j + 16u);
+  for (uint32_t j0 = 0; j0 < rank; j0 += 16u * kDeep) {
+#pragma unroll
+    for (uint32_t d = 0; d < kDeep; ++d)
+      if (j0 + 16u * d < rank) load(step[d], j0 + 16u * d);
+#pragma unroll
+    for (uint32_t d = 0; d < kDeep; ++d)
+      if (j0 + 16u * d < rank) compute(step[d], j0 + 16u * d);
   }
 }
 
