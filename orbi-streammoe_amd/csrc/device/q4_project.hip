@@ -212,7 +212,7 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
       if (w >= p.words) break;  // whole groups of GWS lanes leave together (words is a multiple of GWS)
       float sum = 0.0f;
       f16x8 hi, lo;
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < 8; ++k) {
         constexpr int nibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
         const float s = live ? ldexpf(keep[u].get(nibble[k]), e) : 0.0f;
@@ -734,8 +734,10 @@ template <int XT, int AT, int JB>
 __device__ __forceinline__ void shrink_tile(const ShrinkManyParams& sp, uint32_t block) {
   const ShrinkParams& p = sp.s;
   constexpr int NX = kTerms<XT>, NA = kTerms<AT>;
-  // Steps in flight: within some 100 registers.
-  constexpr int kSteps = JB == 1 ? (XT == OSM_META_F32 || AT == OSM_META_F32 ? 6 : 8) : AT == OSM_META_F32 ? 2 : 4;
+  // Steps in flight, within some 180 registers: one workgroup a compute unit
+  // (fewer in flight or spilled registers for two cost more: 46 us and 53 or
+  // more for 4,096 tokens of 4,096 columns, rank 64).
+  constexpr int kSteps = JB == 1 ? 8 : AT == OSM_META_F32 ? 2 : 4;
   __shared__ float part[kShrinkManyWaves][JB][4][kWave];
   const uint32_t lane = threadIdx.x % kWave, K = p.words * 8u;
   const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / kWave)));
