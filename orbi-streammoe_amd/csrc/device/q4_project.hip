@@ -34,14 +34,18 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ---- the prepared input --------------------------------------------------------
-// The matrix instructions multiply f16 pairs: a nibble q masked in place is
-// the f16 subnormal q 2^-24 (nibbles 0, 2, 4, 6 of a word) or q 2^-20 (1, 3,
-// 5, 7; w & 0x00F000F0), so five instructions unpack eight nibbles, exactly.
+// The matrix instructions multiply f16 pairs: a nibble q in the upper bits of
+// the fraction, below an exponent of 0, is the f16 subnormal q 2^-18, so eight
+// instructions unpack eight nibbles, exactly. (Lower in the fraction they need
+// fewer shifts, but the instructions align products by the operands' exponent
+// fields: a fraction that starts with zeros costs the sum as many bits. In
+// place at q 2^-24 and q 2^-20, five instructions, fp32 outputs of 4,096
+// columns were off by 1e-5.)
 // x is brought to f16 once per call: row t times 2^e, e such that its largest
 // value lies in [2^14, 2^15), as one term (bf16 and f16 input: exact down to
-// 2^-24 steps, 2^-35 of the row's largest value) or as two (fp32: 22 bits),
-// columns that meet a q 2^-20 divided by 16. With D the fp32 sum of a group,
-//   y = 2^(24 - e) sum over groups of (s D + b X),  X = 2^(e - 24) sum of x.
+// 2^-24 steps, 2^-38 of the row's largest value) or as two (fp32: 22 bits).
+// With D the fp32 sum of a group,
+//   y = 2^(18 - e) sum over groups of (s D + b X),  X = 2^(e - 18) sum of x.
 // Products are exact in fp32; nothing else is rounded to fewer bits.
 //
 // Layout: tiles of R tokens in the instructions' operand order. Lane l of an
@@ -59,7 +63,7 @@ constexpr int kAcc = R * R / kWave;  // accumulator registers of one tile
 struct Prepared {
   _Float16* frag;
   float* sums;
-  int32_t* exps;  // 24 - e
+  int32_t* exps;  // 18 - e
   float* v;       // [token][vr] scale_a A_a x, zero from the rank on
   uint32_t vr;    // max_rank rounded up to 16
 };
@@ -202,7 +206,7 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
   }
   if (row >= p.rows) return;
   const int e = 141 - static_cast<int>(__float_as_uint(top) >> 23);
-  if (i == 0) p.out.exps[row] = 24 - e;
+  if (i == 0) p.out.exps[row] = 18 - e;
   const uint32_t tile = row / R, steps = p.words / kSlots<R>, subs = p.words / GWS;
   for (uint32_t w0 = i; w0 < p.words; w0 += kKeep * TPT) {
     if (p.words > kKeep * TPT) batch(w0);
@@ -217,9 +221,8 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
         constexpr int nibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
         const float s = live ? ldexpf(keep[u].get(nibble[k]), e) : 0.0f;
         sum += s;
-        const float o = (nibble[k] & 1) ? s * 0.0625f : s;
-        hi[k] = static_cast<_Float16>(o);
-        if constexpr (NT == 2) lo[k] = static_cast<_Float16>(o - static_cast<float>(hi[k]));
+        hi[k] = static_cast<_Float16>(s);
+        if constexpr (NT == 2) lo[k] = static_cast<_Float16>(s - static_cast<float>(hi[k]));
       }
       const uint32_t sub = w / GWS, iw = w % GWS;
       const uint32_t lane = iw / GW * R + row % R, step = sub * GW + iw % GW;
@@ -229,12 +232,12 @@ __device__ __forceinline__ void prepare_rows(const PrepareParams& p, uint32_t bl
       sum = row_sum<GWS < 16 ? GWS : 16>(sum);
       if constexpr (MANY) {
         if (iw == 0) {
-          store_sum(*many, tile, sub, row % R, sum * 0x1p-24f);
+          store_sum(*many, tile, sub, row % R, sum * 0x1p-18f);
           if (sub + 1u == subs)
             for (uint32_t z = subs; z < many->kgs * 16u; ++z) store_sum(*many, tile, z, row % R, 0.0f);
         }
       } else {
-        if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-24f;
+        if (iw == 0) p.out.sums[(static_cast<size_t>(tile) * subs + sub) * R + row % R] = sum * 0x1p-18f;
       }
     }
   }
@@ -322,8 +325,8 @@ struct Tile<32> {
 
 // Eight nibbles as the operand (see above).
 __device__ __forceinline__ f16x8 nibble_operand(uint32_t w) {
-  const uint32_t t = w >> 8;
-  const u32x4 v = {w & 0x000F000Fu, w & 0x00F000F0u, t & 0x000F000Fu, t & 0x00F000F0u};
+  constexpr uint32_t kMask = 0x03C003C0u;
+  const u32x4 v = {(w << 6) & kMask, (w << 2) & kMask, (w >> 2) & kMask, (w >> 6) & kMask};
   return __builtin_bit_cast(f16x8, v);
 }
 __device__ __forceinline__ f16x8 load_frag(const _Float16* p) { return __builtin_bit_cast(f16x8, ldg<u32x4>(p)); }

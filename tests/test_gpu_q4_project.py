@@ -142,6 +142,19 @@ def test_large_tiles(ctx, T, N, K, group, x):
         Problem(ctx, T, N, K, group, meta, x, count=5 if meta == BF16 else 0, rank=24, ragged=True, y_pad=8 * (meta == F16)).check()
 
 
+# fp32 in and out: the outputs' rms error is at most that of one fp32 sum over the columns in turn. Each of its K roundings is
+# 2^-25 rms of a partial sum, which grows as the square root of its terms: together 2^-25 sqrt(K / 2) of the result.
+@pytest.mark.parametrize("T,N", [(1, 512), (12, 256), (37, 256), (64, 8192), (100, 256), (2048, 4096)])
+@pytest.mark.parametrize("K,group", [(2048, 32), (4096, 64), (4096, 128)])
+def test_sums_are_fp32(ctx, T, N, K, group):
+    print(f"[project] T={T} N={N} K={K} group={group}", flush=True)
+    for x in (F32, F16, BF16):
+        for count in (0, 4):
+            p = Problem(ctx, T, N, K, group, F32, x, y=F32, count=count, rank=16, adapter=F32)
+            off = p.run() - p.y64
+            assert np.sqrt(np.mean(off**2) / np.mean(p.y64**2)) <= 2.0**-25 * np.sqrt(K / 2)
+
+
 def test_more_adapters_than_are_sorted(ctx):
     for x in (F32, BF16):
         for T in (3, 30, 130):
