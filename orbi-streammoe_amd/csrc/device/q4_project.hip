@@ -299,9 +299,12 @@ __global__ __launch_bounds__(256) void prepare_few_kernel(PrepareParams p, Shrin
 
 // ---- few tokens ------------------------------------------------------------------
 // A workgroup owns R rows of W and R tokens; its wavefronts split the columns
-// and their sums are added in LDS in wavefront order. The
-// lanes of an instruction's D columns are rows of W, so a lane needs one
-// scale and bias per sub-group.
+// and their sums are added in LDS in wavefront order. The lanes of an
+// instruction's D columns are rows of W, so a lane needs one scale and bias
+// per sub-group. What bounds it is the latency of one stage (words, then the
+// sums, then the adapters' rows): 37 fp32 tokens through 2048 x 4096 take 5 us
+// of preparation and 12 here, 64 bf16 ones through 12289 x 2048 take 5 and 23
+// (35 MB, 25 of them B_a of 64 adapters: 1.5 TB/s).
 template <int R>
 struct Tile;
 template <>
@@ -561,7 +564,8 @@ __global__ __launch_bounds__(kFewWaves* kWave, 4) void project_few_kernel(Projec
 // ---- one to four tokens ----------------------------------------------------------
 // A wavefront takes ROWS rows of W; a lane holds 32 consecutive columns of
 // each token in registers (a chunk, within one quantisation group) and the
-// chunk's sum for the bias. No preparation: one launch, after the shrink.
+// chunk's sum for the bias. No preparation: one launch, after the shrink (2.6
+// us; 4096 x 2048 for one token then takes 5.4, 4.9 MB).
 constexpr int kVecWaves = 4;
 
 template <int XT>
@@ -648,6 +652,10 @@ __global__ __launch_bounds__(kVecWaves* kWave) void project_vec_kernel(VecParams
 // three; a bias into one, two or three by its type), products below 2^-24 of
 // the whole left out. Before the main launch one prepares x (as above), the
 // scales transposed to [sub-group][row] and the biases as operands.
+// 4,096 bf16 tokens through 8192 x 4096, rank 64: 345 to 354 us here (281 GFLOP, 800
+// TFLOP/s; the slope is 63 us per 1,024 columns, so some 80 are a tile's
+// beginning and end, where a compute unit has nothing else to run) and 46 + 5
+// before it, which are the first products' loads from L2 and x's round trip.
 template <int AT>
 constexpr int kTerms = AT == OSM_META_BF16 ? 1 : AT == OSM_META_F16 ? 2 : 3;  // exact in that many bf16 terms
 
@@ -1527,21 +1535,21 @@ int launch_many(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipSt
   // The tile with the least time expected: microseconds of a round of
   // workgroups at 2,048 columns (the others' in proportion) times the rounds.
   // One term, tiles of 64 x 128 / 128 x 128 / 128 x 256, measured: 512 tokens
-  // through 4,096 rows 16 / 26 / 33, 1,024: 29 / 29 / 36, 2,048: 59 / 45 / 42.
-  // Two terms, 32 x 128 / 128 x 256: 31 / 74, 59 / 76, 130 / 94.
+  // through 4,096 rows 17 / 27 / 35, 1,024: 32 / 30 / 38, 2,048: 65 / 47 / 44.
+  // Two terms, 32 x 128 / 128 x 256: 32 / 84, 62 / 88, 132 / 105.
   auto groups = [&](uint32_t tiles, uint32_t rows) {
     return (mp.tiles + tiles - 1u) / tiles * ((a.w.out_dim + rows - 1u) / rows);
   };
   return by_dtype(a.w.meta_dtype, [&](auto meta) {
     constexpr int M = decltype(meta)::value;
     if (pl.terms == 2u) {
-      if ((groups(1u, 128u) + 255u) / 256u * 15u <= (groups(4u, 256u) + 255u) / 256u * 92u)
+      if ((groups(1u, 128u) + 255u) / 256u * 16u <= (groups(4u, 256u) + 255u) / 256u * 102u)
         return go(project_many_kernel<M, 2, 1, 1, 1, 4, 2, GW, 256, 3>, 1u, 128u, 512u);
       return go(project_many_kernel<M, 2, 2, 2, 2, 4, 1, GW, 64, 3>, 4u, 256u, 512u);
     }
-    const uint32_t small = (groups(2u, 128u) + 255u) / 256u * 15u;
-    const uint32_t middle = groups(4u, 128u) <= 256u ? 26u : (groups(4u, 128u) + 511u) / 512u * 45u;
-    const uint32_t large = (groups(4u, 256u) + 255u) / 256u * 41u;
+    const uint32_t small = (groups(2u, 128u) + 255u) / 256u * 16u;
+    const uint32_t middle = groups(4u, 128u) <= 256u ? 28u : (groups(4u, 128u) + 511u) / 512u * 47u;
+    const uint32_t large = (groups(4u, 256u) + 255u) / 256u * 43u;
     if (small <= middle && small <= large) return go(project_many_kernel<M, 1, 1, 1, 2, 4, 1, GW, 128, 4>, 2u, 128u, 512u);
     if (middle <= large) return go(project_many_kernel<M, 1, 2, 2, 2, 2, 1, GW, 64, 3>, 4u, 128u, 256u);
     return go(project_many_kernel<M, 1, 2, 2, 2, 4, 1, GW, 64, 3>, 4u, 256u, 512u);
