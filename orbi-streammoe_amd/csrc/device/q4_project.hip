@@ -1296,7 +1296,7 @@ constexpr int kShrinkWaves = 4;
 // v[t, j] = scale_a (A_a x_t)_j: a wavefront per rank row and token.
 template <int XT, int AT>
 __global__ __launch_bounds__(kShrinkWaves* kWave) void shrink_kernel(ShrinkParams p) {
-  shrink_rows<XT, AT>(p, blockIdx.x);
+  for (uint32_t block = blockIdx.x; block < p.tokens * (p.vr / kShrinkWaves); block += gridDim.x) shrink_rows<XT, AT>(p, block);
 }
 
 constexpr int kAnyWaves = 4;
@@ -1463,10 +1463,10 @@ ProjectParams project_params(const osmd_project_args& a, const Plan& pl, uint8_t
 
 int launch_shrink(const osmd_project_args& a, const Plan& pl, uint8_t* work, hipStream_t st) {
   const ShrinkParams sp = shrink_params(a, pl, work);
+  const uint32_t blocks = a.tokens * (pl.vr / kShrinkWaves), grid = blocks < 1u << 20 ? blocks : 1u << 20;
   return by_dtype(a.x_dtype, [&](auto xt) {
     return by_dtype(a.adapters.dtype, [&](auto at) {
-      shrink_kernel<decltype(xt)::value, decltype(at)::value>
-          <<<a.tokens * (pl.vr / kShrinkWaves), kShrinkWaves * kWave, 0, st>>>(sp);
+      shrink_kernel<decltype(xt)::value, decltype(at)::value><<<grid, kShrinkWaves * kWave, 0, st>>>(sp);
       return launch_status();
     });
   });

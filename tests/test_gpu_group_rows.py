@@ -46,6 +46,34 @@ def test_matches_stable_sort(ctx, n, buckets):
         assert np.array_equal(order, ref_order), name
 
 
+def test_many_rows_in_a_capture(ctx):
+    # The counts of many rows are in the context's workspace: it does not grow while a capture is recording.
+    rng = np.random.default_rng(3)
+    fresh = osm_hip.Context(0)
+    n, buckets = 50001, 300
+    keys, offsets, order = fresh.alloc(4 * n), fresh.alloc(4 * (buckets + 1)), fresh.alloc(4 * n)
+    with fresh.capture() as small:
+        with pytest.raises(osm_hip.OsmError) as e:
+            osm_hip.group_rows(fresh, keys.ptr, n, buckets, offsets.ptr, order.ptr)
+        osm_hip.group_rows(fresh, keys.ptr, 9, 1, offsets.ptr, order.ptr)
+    assert "capture" in e.value.diagnostic
+    keys.upload(np.zeros(n, np.int32))
+    small.graph.launch()
+    osm_hip.group_rows(fresh, keys.ptr, n, buckets, offsets.ptr, order.ptr)
+    with fresh.capture() as cap:
+        osm_hip.group_rows(fresh, keys.ptr, n, buckets, offsets.ptr, order.ptr)
+    for _ in range(3):
+        k = rng.integers(-1, buckets + 1, n).astype(np.int32)
+        keys.upload(k)
+        cap.graph.launch()
+        fresh.synchronize()
+        ref_offsets, ref_order = expected(k, buckets)
+        assert np.array_equal(offsets.download(np.uint32, buckets + 1), ref_offsets)
+        assert np.array_equal(order.download(np.uint32, n), ref_order)
+        assert np.array_equal(group(fresh, k[::-1].copy(), 7)[1], expected(k[::-1], 7)[1])  # other work in the same workspace
+    fresh.close()
+
+
 def test_refused(ctx):
     a = ctx.alloc(256)
     odd = ctypes.c_void_p(a.ptr.value + 2)

@@ -155,6 +155,15 @@ def test_sums_are_fp32(ctx, T, N, K, group):
             assert np.sqrt(np.mean(off**2) / np.mean(p.y64**2)) <= 2.0**-25 * np.sqrt(K / 2)
 
 
+def test_as_many_tokens_as_a_call_takes(ctx):
+    T = 1 << 20
+    ids = np.full(T, -1)
+    ids[[0, 1, 70001, T - 2, T - 1]] = 0, 1, 1, 1, 0
+    for N, K, group, rank in ((1, 8, 8, 64), (32, 32, 32, 8)):
+        print(f"[project] T={T} N={N} K={K} group={group}", flush=True)
+        Problem(ctx, T, N, K, group, BF16, BF16, count=2, rank=rank, ids=ids).check()
+
+
 def test_more_adapters_than_are_sorted(ctx):
     for x in (F32, BF16):
         for T in (3, 30, 130):
