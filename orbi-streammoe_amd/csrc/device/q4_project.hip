@@ -259,19 +259,29 @@ __device__ __forceinline__ void shrink_rows(const ShrinkParams& p, uint32_t bloc
   const uint32_t blocks = p.vr / 4u;
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const uint32_t t = block / blocks, j = block % blocks * 4u + wave;
+  constexpr uint32_t kAhead = 4;  // pieces of 8 columns in flight
+  const size_t xo = t * p.stride;
+  Raw8<XT> x[kAhead];
+  auto load_x = [&](uint32_t w0) {
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) {
+      const uint32_t w = w0 + u * kWave < p.words ? w0 + u * kWave : p.words - 1u;
+      load_raw8<XT>(p.x, xo + 8u * w, p.x_wide, x[u]);
+    }
+  };
+  load_x(lane);  // while the adapter's id and rank are on their way
   uint32_t a = 0;
   const uint32_t rank = token_rank(p.ad, p.ids, t, a);
   float s = 0.0f;
   if (j < rank) {
-    const size_t xo = t * p.stride, ao = (static_cast<size_t>(a) * p.ad.max_rank + j) * p.words * 8u;
-    constexpr uint32_t kAhead = 4;  // pieces of 8 columns in flight
+    const float scale = p.ad.scales ? p.ad.scales[a] : 1.0f;
+    const size_t ao = (static_cast<size_t>(a) * p.ad.max_rank + j) * p.words * 8u;
     for (uint32_t w0 = lane; w0 < p.words; w0 += kAhead * kWave) {
-      Raw8<XT> x[kAhead];
+      if (w0 != lane) load_x(w0);
       Raw8<AT> c[kAhead];
 #pragma unroll
       for (uint32_t u = 0; u < kAhead; ++u) {
-        const uint32_t w = w0 + u * kWave < p.words ? w0 + u * kWave : w0;
-        load_raw8<XT>(p.x, xo + 8u * w, p.x_wide, x[u]);
+        const uint32_t w = w0 + u * kWave < p.words ? w0 + u * kWave : p.words - 1u;
         load_raw8<AT>(p.ad.a, ao + 8u * w, p.a_wide, c[u]);
       }
 #pragma unroll
@@ -282,8 +292,7 @@ __device__ __forceinline__ void shrink_rows(const ShrinkParams& p, uint32_t bloc
         s += w0 + u * kWave < p.words ? d : 0.0f;
       }
     }
-    s = wave_sum(s);
-    if (p.ad.scales) s *= p.ad.scales[a];
+    s = wave_sum(s) * scale;
   }
   if (lane == 0) p.v[static_cast<size_t>(t) * p.vr + j] = s;
 }
@@ -564,7 +573,7 @@ __global__ __launch_bounds__(kFewWaves* kWave, 4) void project_few_kernel(Projec
 // ---- one to four tokens ----------------------------------------------------------
 // A wavefront takes ROWS rows of W; a lane holds 32 consecutive columns of
 // each token in registers (a chunk, within one quantisation group) and the
-// chunk's sum for the bias. No preparation: one launch, after the shrink (2.6
+// chunk's sum for the bias. No preparation: one launch, after the shrink (2.4
 // us; 4096 x 2048 for one token then takes 5.4, 4.9 MB).
 constexpr int kVecWaves = 4;
 
@@ -593,6 +602,23 @@ __global__ __launch_bounds__(kVecWaves* kWave) void project_vec_kernel(VecParams
   const uint32_t N = p.w.out_dim, words = p.w.packed_cols, chunks = words / 4u, G = p.w.group;
   const uint32_t n0 = (blockIdx.x * kVecWaves + wave) * ROWS, t0 = blockIdx.y * TV;
   if (n0 >= N) return;
+  // The adapters' columns, one a lane, join the lanes' sums; the first 64 are
+  // loaded before the weights.
+  uint32_t a[TV] = {}, rank[TV];
+  float column[ROWS][TV], v[TV];
+  auto load_columns = [&](int t, uint32_t j) {
+    v[t] = p.in.v[static_cast<size_t>(t0 + t) * p.in.vr + j];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const size_t n = n0 + r < N ? n0 + r : N - 1u;
+      column[r][t] = adapter_element(p.ad, (a[t] * static_cast<size_t>(N) + n) * p.ad.max_rank + j);
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < TV; ++t) {
+    rank[t] = t0 + t < p.tokens ? token_rank(p.ad, p.ids, t0 + t, a[t]) : 0u;
+    if (lane < rank[t]) load_columns(t, lane);
+  }
   float acc[ROWS][TV] = {};
   for (uint32_t c = lane; c < chunks; c += kWave) {
     uint4 q[ROWS];
@@ -618,20 +644,13 @@ __global__ __launch_bounds__(kVecWaves* kWave) void project_vec_kernel(VecParams
       for (int t = 0; t < TV; ++t)
         acc[r][t] = fmaf(meta_widen<META>(sb[r]), nib_dot32(q[r], x[t]), fmaf(meta_widen<META>(bb[r]), sum[t], acc[r][t]));
   }
-  // The adapters' columns, one a lane, join the lanes' sums.
 #pragma unroll
-  for (int t = 0; t < TV; ++t) {
-    uint32_t a = 0;
-    const uint32_t rank = t0 + t < p.tokens ? token_rank(p.ad, p.ids, t0 + t, a) : 0u;
-    for (uint32_t j = lane; j < rank; j += kWave) {
-      const float v = p.in.v[static_cast<size_t>(t0 + t) * p.in.vr + j];
+  for (int t = 0; t < TV; ++t)
+    for (uint32_t j = lane; j < rank[t]; j += kWave) {
+      if (j != lane) load_columns(t, j);
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const size_t n = n0 + r < N ? n0 + r : N - 1u;
-        acc[r][t] = fmaf(adapter_element(p.ad, (a * static_cast<size_t>(N) + n) * p.ad.max_rank + j), v, acc[r][t]);
-      }
+      for (int r = 0; r < ROWS; ++r) acc[r][t] = fmaf(column[r][t], v[t], acc[r][t]);
     }
-  }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
