@@ -574,7 +574,7 @@ __global__ __launch_bounds__(kFewWaves* kWave, 4) void project_few_kernel(Projec
 // A wavefront takes ROWS rows of W; a lane holds 32 consecutive columns of
 // each token in registers (a chunk, within one quantisation group) and the
 // chunk's sum for the bias. No preparation: one launch, after the shrink (2.4
-// us; 4096 x 2048 for one token then takes 5.4, 4.9 MB).
+// us; 4096 x 2048 for one token then takes 5.2 to 5.6, 4.9 MB).
 constexpr int kVecWaves = 4;
 
 template <int XT>
